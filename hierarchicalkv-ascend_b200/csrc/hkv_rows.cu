@@ -1,0 +1,659 @@
+// hkv_rows.cu -- tokens sorted by group (expert, table, owner) and back with
+// weights, and the gradients of both ways.
+//
+// All kernels move rows by an index list and are bound by memory: the floor is
+// the bytes of the ids, positions and rows at the copy bandwidth. Sums are held
+// in float32 and rounded once.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <string>
+#include <type_traits>
+
+#include "hkv_table.cuh"
+
+namespace hkvb {
+
+void set_last_error(const std::string& m);
+
+namespace {
+
+// q = n / d for n < 2^31: with 2^c >= d and m = ceil(2^(31 + c) / d), the
+// error m * d - 2^(31 + c) is below d <= 2^c, so n * error / 2^(31 + c) / d
+// stays below 1 / d and the floor is exact.
+struct FastDiv {
+  uint32_t d, m, s;
+  explicit FastDiv(uint32_t d_) : d(d_), m(0), s(0) {
+    if (d == 1) return;
+    uint32_t c = 0;
+    while ((1ull << c) < d) c++;
+    m = static_cast<uint32_t>(((1ull << (31 + c)) + d - 1) / d);
+    s = c - 1;
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    return d == 1 ? n : __umulhi(n, m) >> s;
+  }
+};
+
+// ---- sort by group ----------------------------------------------------------
+
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortItems = 8;  // places of a thread and tile
+constexpr int kSortTile = kSortThreads * kSortItems;
+constexpr uint32_t kSortBlocks = 592;  // 4 x 148: blocks of the long form
+
+template <class Id>
+__device__ __forceinline__ int load_group(const void* groups, uint64_t i, uint64_t n,
+                                          uint32_t num_groups) {
+  if (i >= n) return -1;
+  const Id id = static_cast<const Id*>(groups)[i];
+  return id >= 0 && id < static_cast<Id>(num_groups) ? static_cast<int>(id) : -1;
+}
+
+// Exclusive sum of v over the block's threads, and the sum of all.
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* warp_sums,
+                                                    uint32_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  uint32_t inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(~0u, inc, o);
+    if (lane >= o) inc += u;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = inc;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+  for (int w = 0; w < warps; w++) {
+    const uint32_t u = warp_sums[w];
+    if (w < warp) before += u;
+    all += u;
+  }
+  *total = all;
+  return before + inc - v;
+}
+
+// counts[g * blocks + b]: the places of group g in block b's run of tiles
+template <class Id>
+__global__ void __launch_bounds__(kSortThreads)
+    group_count_kernel(uint64_t n, const void* groups, uint32_t num_groups,
+                       uint32_t tiles_per_block, uint32_t* counts) {
+  extern __shared__ uint32_t hist[];
+  for (uint32_t g = threadIdx.x; g < num_groups; g += blockDim.x) hist[g] = 0;
+  __syncthreads();
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * tiles_per_block * kSortTile;
+  const uint64_t last = min(n, first + static_cast<uint64_t>(tiles_per_block) * kSortTile);
+  const uint32_t below = (1u << (threadIdx.x & 31)) - 1;
+  for (uint64_t base = first; base < last; base += kSortThreads) {
+    const int id = load_group<Id>(groups, base + threadIdx.x, last, num_groups);
+    const uint32_t same = __match_any_sync(~0u, id);
+    if (id >= 0 && (same & below) == 0) atomicAdd(&hist[id], __popc(same));
+  }
+  __syncthreads();
+  for (uint32_t g = threadIdx.x; g < num_groups; g += blockDim.x)
+    counts[static_cast<uint64_t>(g) * gridDim.x + blockIdx.x] = hist[g];
+}
+
+// a warp per group: its counts become the places in earlier blocks, and the sum
+__global__ void group_scan_kernel(uint32_t num_groups, uint32_t blocks, uint32_t* counts,
+                                  uint32_t* totals) {
+  const uint32_t g = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (g >= num_groups) return;
+  uint32_t* c = counts + static_cast<uint64_t>(g) * blocks;
+  uint32_t run = 0;
+  for (uint32_t b = 0; b < blocks; b += 32) {
+    const uint32_t v = b + lane < blocks ? c[b + lane] : 0;
+    uint32_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(~0u, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (b + lane < blocks) c[b + lane] = run + inc - v;
+    run += __shfl_sync(~0u, inc, 31);
+  }
+  if (lane == 0) totals[g] = run;
+}
+
+// Ranks the places of a block's tiles. A warp takes a run of 32 * kSortItems
+// places; __match_any_sync gives each place its rank among the equal ids of its
+// warp step, the warp's count of the id what came before. The counts of the
+// block's warps, scanned over the warps, and the start of the group make the
+// row.
+template <class Id>
+__global__ void __launch_bounds__(kSortThreads)
+    group_place_kernel(uint64_t n, const void* groups, uint32_t num_groups,
+                       uint32_t tiles_per_block, const uint32_t* counts,
+                       const uint32_t* totals, int32_t* offsets, int32_t* positions,
+                       int32_t* order) {
+  extern __shared__ uint32_t smem[];
+  __shared__ uint32_t warp_sums[32];
+  uint32_t* start = smem;  // [num_groups]
+  uint16_t* cnt = reinterpret_cast<uint16_t*>(smem + num_groups);  // [kSortWarps + 1][num_groups]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t below = (1u << lane) - 1;
+
+  // start of each group, over contiguous runs of groups per thread
+  const uint32_t per = (num_groups + kSortThreads - 1) / kSortThreads;
+  const uint32_t g0 = min(num_groups, threadIdx.x * per), g1 = min(num_groups, g0 + per);
+  uint32_t sum = 0, kept = 0;
+  for (uint32_t g = g0; g < g1; g++) sum += totals[g];
+  uint32_t run = block_exclusive(sum, warp_sums, &kept);
+  for (uint32_t g = g0; g < g1; g++) {
+    if (blockIdx.x == 0) offsets[g] = run;
+    start[g] = run + counts[static_cast<uint64_t>(g) * gridDim.x + blockIdx.x];
+    run += totals[g];
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) offsets[num_groups] = kept;
+
+  if (order != nullptr)  // places without a row
+    for (uint64_t i = kept + blockIdx.x * static_cast<uint64_t>(kSortThreads) + threadIdx.x; i < n;
+         i += static_cast<uint64_t>(gridDim.x) * kSortThreads)
+      order[i] = -1;
+
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * tiles_per_block;
+  for (uint32_t t = 0; t < tiles_per_block; t++) {
+    const uint64_t base = (first + t) * kSortTile + warp * 32 * kSortItems;
+    if ((first + t) * kSortTile >= n) break;
+    for (uint32_t k = threadIdx.x; k < num_groups * kSortWarps; k += kSortThreads) cnt[k] = 0;
+    __syncthreads();
+    int id[kSortItems];
+    uint32_t rank[kSortItems];
+#pragma unroll
+    for (int it = 0; it < kSortItems; it++)
+      id[it] = load_group<Id>(groups, base + it * 32 + lane, n, num_groups);
+    uint16_t* mine = cnt + warp * num_groups;
+#pragma unroll
+    for (int it = 0; it < kSortItems; it++) {
+      const uint32_t same = __match_any_sync(~0u, id[it]);
+      const uint32_t before = id[it] >= 0 ? mine[id[it]] : 0;
+      rank[it] = before + __popc(same & below);
+      __syncwarp();
+      if (id[it] >= 0 && (same & below) == 0) mine[id[it]] = before + __popc(same);
+      __syncwarp();
+    }
+    __syncthreads();
+    for (uint32_t g = threadIdx.x; g < num_groups; g += kSortThreads) {
+      uint32_t before = 0;
+      for (int w = 0; w < kSortWarps; w++) {
+        const uint32_t c = cnt[w * num_groups + g];
+        cnt[w * num_groups + g] = before;
+        before += c;
+      }
+      cnt[kSortWarps * num_groups + g] = before;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int it = 0; it < kSortItems; it++) {
+      const uint64_t i = base + it * 32 + lane;
+      if (i >= n) continue;
+      if (id[it] < 0) {
+        positions[i] = -1;
+        continue;
+      }
+      const uint32_t row = start[id[it]] + mine[id[it]] + rank[it];
+      positions[i] = row;
+      if (order != nullptr) order[row] = static_cast<int32_t>(i);
+    }
+    __syncthreads();
+    for (uint32_t g = threadIdx.x; g < num_groups; g += kSortThreads)
+      start[g] += cnt[kSortWarps * num_groups + g];
+  }
+}
+
+uint32_t sort_tiles_per_block(size_t n) {
+  const size_t tiles = (n + kSortTile - 1) / kSortTile;
+  return static_cast<uint32_t>(std::max<size_t>(1, (tiles + kSortBlocks - 1) / kSortBlocks));
+}
+
+uint32_t sort_blocks(size_t n) {
+  const size_t run = static_cast<size_t>(sort_tiles_per_block(n)) * kSortTile;
+  return static_cast<uint32_t>(std::max<size_t>(1, (n + run - 1) / run));
+}
+
+size_t sort_workspace(size_t n, uint32_t num_groups) {
+  return (static_cast<size_t>(num_groups) * sort_blocks(n) + num_groups) * 4;
+}
+
+template <class Id>
+void launch_sort(size_t n, const void* groups, uint32_t num_groups, int32_t* offsets,
+                 int32_t* positions, int32_t* order, void* workspace, cudaStream_t s) {
+  const uint32_t blocks = sort_blocks(n), run = sort_tiles_per_block(n);
+  uint32_t* counts = static_cast<uint32_t*>(workspace);
+  uint32_t* totals = counts + static_cast<size_t>(num_groups) * blocks;
+  group_count_kernel<Id><<<blocks, kSortThreads, num_groups * 4, counted(s)>>>(
+      n, groups, num_groups, run, counts);
+  CUDA_TRY(cudaGetLastError());
+  group_scan_kernel<<<(num_groups + 7) / 8, 256, 0, counted(s)>>>(num_groups, blocks, counts,
+                                                                  totals);
+  CUDA_TRY(cudaGetLastError());
+  const size_t smem = num_groups * (4 + 2 * (kSortWarps + 1));
+  if (smem > 48 * 1024)
+    CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<Id>,
+                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>(smem)));
+  group_place_kernel<Id><<<blocks, kSortThreads, smem, counted(s)>>>(
+      n, groups, num_groups, run, counts, totals, offsets, positions, order);
+  CUDA_TRY(cudaGetLastError());
+}
+
+// ---- rows -------------------------------------------------------------------
+
+constexpr int kRowThreads = 256;
+
+template <int kBytes>
+struct Word;
+template <> struct Word<16> { using type = uint4; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<2> { using type = uint16_t; };
+template <> struct Word<1> { using type = uint8_t; };
+
+// A thread reads one word of a token's row once and writes it to every place's
+// row. Strides in words.
+template <int kBytes>
+__global__ void __launch_bounds__(kRowThreads)
+    dispatch_kernel(uint32_t words_of_all, FastDiv words, uint32_t slots, const void* x,
+                    uint64_t x_stride, const int32_t* positions, uint32_t num_rows, void* rows,
+                    uint64_t rows_stride) {
+  using T = typename Word<kBytes>::type;
+  const uint32_t i = blockIdx.x * kRowThreads + threadIdx.x;
+  if (i >= words_of_all) return;
+  const uint32_t t = words.div(i), c = i - t * words.d;
+  const T v = static_cast<const T*>(x)[t * x_stride + c];
+  const int32_t* p = positions + static_cast<uint64_t>(t) * slots;
+  for (uint32_t k = 0; k < slots; k++) {
+    const uint32_t row = static_cast<uint32_t>(p[k]);
+    if (row < num_rows) static_cast<T*>(rows)[row * rows_stride + c] = v;
+  }
+}
+
+template <class T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float(float v) { return v; }
+template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <class T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// kVec elements of a row: 16 bytes where rows are aligned to that, else one
+template <class T, int kVec>
+struct alignas(sizeof(T) * kVec) Pack {
+  T v[kVec];
+};
+
+// A thread sums one pack of a token's output over its slots.
+template <class T, class W, int kVec>
+__global__ void __launch_bounds__(kRowThreads)
+    combine_kernel(uint32_t packs_of_all, FastDiv packs, uint32_t slots, const T* rows,
+                   uint64_t rows_stride, uint32_t num_rows, const int32_t* positions,
+                   const W* weights, T* out, uint64_t out_stride) {
+  const uint32_t i = blockIdx.x * kRowThreads + threadIdx.x;
+  if (i >= packs_of_all) return;
+  const uint32_t t = packs.div(i), c = (i - t * packs.d) * kVec;
+  const uint64_t place = static_cast<uint64_t>(t) * slots;
+  float acc[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; e++) acc[e] = 0.f;
+  for (uint32_t k = 0; k < slots; k++) {
+    const uint32_t row = positions ? static_cast<uint32_t>(positions[place + k])
+                                   : static_cast<uint32_t>(place + k);
+    if (row >= num_rows) continue;
+    const float w = weights ? to_float(weights[place + k]) : 1.f;
+    const auto v = *reinterpret_cast<const Pack<T, kVec>*>(rows + row * rows_stride + c);
+#pragma unroll
+    for (int e = 0; e < kVec; e++) acc[e] = fmaf(w, to_float(v.v[e]), acc[e]);
+  }
+  Pack<T, kVec> o;
+#pragma unroll
+  for (int e = 0; e < kVec; e++) o.v[e] = from_float<T>(acc[e]);
+  *reinterpret_cast<Pack<T, kVec>*>(out + t * out_stride + c) = o;
+}
+
+// kLanes lanes per place: the row of the gradient, and the inner product in
+// per-lane sums joined by a fixed tree of shuffles.
+template <class T, class W, int kVec, int kLanes>
+__global__ void __launch_bounds__(kRowThreads)
+    combine_backward_kernel(uint32_t places, FastDiv slots, uint32_t packs, const T* rows,
+                            uint64_t rows_stride, uint32_t num_rows, const int32_t* positions,
+                            const W* weights, const T* grad_out, uint64_t grad_out_stride,
+                            T* grad_rows, uint64_t grad_rows_stride, W* grad_weights) {
+  const uint32_t i = (blockIdx.x * static_cast<uint64_t>(kRowThreads) + threadIdx.x) / kLanes;
+  const uint32_t lane = threadIdx.x % kLanes;
+  const bool on = i < places;
+  const uint32_t row = !on ? ~0u : positions ? static_cast<uint32_t>(positions[i]) : i;
+  const bool has = row < num_rows;
+  float dot = 0.f;
+  if (has) {
+    const float w = weights ? to_float(weights[i]) : 1.f;
+    const T* g = grad_out + slots.div(i) * grad_out_stride;
+    const T* y = rows + row * rows_stride;
+    T* gy = grad_rows + row * grad_rows_stride;
+    for (uint32_t p = lane; p < packs; p += kLanes) {
+      const auto gv = *reinterpret_cast<const Pack<T, kVec>*>(g + p * kVec);
+      if (grad_weights) {
+        const auto yv = *reinterpret_cast<const Pack<T, kVec>*>(y + p * kVec);
+#pragma unroll
+        for (int e = 0; e < kVec; e++) dot = fmaf(to_float(gv.v[e]), to_float(yv.v[e]), dot);
+      }
+      if (grad_rows) {
+        Pack<T, kVec> o;
+#pragma unroll
+        for (int e = 0; e < kVec; e++) o.v[e] = from_float<T>(w * to_float(gv.v[e]));
+        *reinterpret_cast<Pack<T, kVec>*>(gy + p * kVec) = o;
+      }
+    }
+  }
+  if (grad_weights) {
+#pragma unroll
+    for (int o = kLanes / 2; o; o >>= 1) dot += __shfl_xor_sync(~0u, dot, o, kLanes);
+    if (on && lane == 0) grad_weights[i] = from_float<W>(dot);
+  }
+}
+
+// ---- host -------------------------------------------------------------------
+
+uint32_t type_bytes(int vt) {
+  switch (vt) {
+    case HKV_VALUE_F32: case HKV_VALUE_U32: return 4;
+    case HKV_VALUE_F16: case HKV_VALUE_BF16: case HKV_VALUE_U16: return 2;
+    case HKV_VALUE_F64: case HKV_VALUE_U64: return 8;
+    case HKV_VALUE_I8: return 1;
+    default: return 0;
+  }
+}
+
+constexpr size_t kMaxCount = 0x7fffffff;
+
+struct RowShape {
+  size_t n, slots, dim;
+  uint32_t bytes;  // of an element
+};
+
+RowShape check_shape(size_t n, size_t slots, size_t dim, int value_type, size_t num_rows) {
+  RowShape r{n, slots, dim, type_bytes(value_type)};
+  HKV_REQUIRE(r.bytes != 0, HKV_ERR_INVALID, "unknown value type");
+  HKV_REQUIRE(slots > 0 && dim > 0, HKV_ERR_INVALID, "slots and dim must be positive");
+  HKV_REQUIRE(slots <= kMaxCount && dim <= kMaxCount && n <= kMaxCount / slots, HKV_ERR_INVALID,
+              "n * slots and dim must be below 2^31");
+  HKV_REQUIRE(num_rows <= kMaxCount, HKV_ERR_INVALID, "num_rows must be below 2^31");
+  return r;
+}
+
+uint64_t stride_or(size_t stride, size_t dim, const char* what) {
+  HKV_REQUIRE(stride == 0 || stride >= dim, HKV_ERR_INVALID,
+              std::string(what) + " must be 0 or at least dim");
+  return stride ? stride : dim;
+}
+
+void require(const void* p, size_t align, const char* what) {
+  HKV_REQUIRE(p != nullptr, HKV_ERR_INVALID, std::string(what) + " is null");
+  HKV_REQUIRE(reinterpret_cast<uintptr_t>(p) % align == 0, HKV_ERR_INVALID,
+              std::string(what) + " is not aligned to its elements");
+}
+
+// largest word (16 bytes at most) that addresses, strides and rows are
+// multiples of
+uint32_t word_bytes(std::initializer_list<const void*> ptrs, std::initializer_list<uint64_t> sizes) {
+  uint64_t all = 16;
+  for (const void* p : ptrs) all |= reinterpret_cast<uintptr_t>(p);
+  for (uint64_t b : sizes) all |= b;
+  return static_cast<uint32_t>(all & (~all + 1));
+}
+
+// Slices of tokens whose words or packs stay below 2^31, for 32-bit indexes.
+template <class F>
+void in_slices(size_t n, size_t per_token, F f) {
+  const size_t step = std::max<size_t>(1, kMaxCount / per_token);
+  for (size_t t = 0; t < n; t += step) f(t, std::min(step, n - t));
+}
+
+uint32_t blocks_for(size_t threads) {
+  return static_cast<uint32_t>((threads + kRowThreads - 1) / kRowThreads);
+}
+
+template <int kBytes>
+void launch_dispatch(const RowShape& r, const void* x, uint64_t x_stride,
+                     const int32_t* positions, size_t num_rows, void* rows,
+                     uint64_t rows_stride, cudaStream_t s) {
+  const uint32_t words = static_cast<uint32_t>(r.dim * r.bytes / kBytes);
+  in_slices(r.n, words, [&](size_t t, size_t m) {
+    dispatch_kernel<kBytes><<<blocks_for(m * words), kRowThreads, 0, counted(s)>>>(
+        static_cast<uint32_t>(m * words), FastDiv(words), static_cast<uint32_t>(r.slots),
+        static_cast<const uint8_t*>(x) + t * x_stride * r.bytes, x_stride * r.bytes / kBytes,
+        positions + t * r.slots, static_cast<uint32_t>(num_rows), rows,
+        rows_stride * r.bytes / kBytes);
+    CUDA_TRY(cudaGetLastError());
+  });
+}
+
+template <class T, class W, int kVec>
+void launch_combine(const RowShape& r, const void* rows, uint64_t rows_stride, size_t num_rows,
+                    const int32_t* positions, const void* weights, void* out,
+                    uint64_t out_stride, cudaStream_t s) {
+  const uint32_t packs = static_cast<uint32_t>(r.dim / kVec);
+  in_slices(r.n, packs, [&](size_t t, size_t m) {
+    // without positions the rows go by place: those of the slice begin at t * slots
+    const size_t skip = positions ? 0 : t * r.slots;
+    if (skip > num_rows) num_rows = skip;
+    combine_kernel<T, W, kVec><<<blocks_for(m * packs), kRowThreads, 0, counted(s)>>>(
+        static_cast<uint32_t>(m * packs), FastDiv(packs), static_cast<uint32_t>(r.slots),
+        static_cast<const T*>(rows) + skip * rows_stride, rows_stride,
+        static_cast<uint32_t>(num_rows - skip), positions ? positions + t * r.slots : nullptr,
+        weights ? static_cast<const W*>(weights) + t * r.slots : nullptr,
+        static_cast<T*>(out) + t * out_stride, out_stride);
+    CUDA_TRY(cudaGetLastError());
+  });
+}
+
+template <class T, class W, int kVec, int kLanes>
+void launch_backward(const RowShape& r, const void* rows, uint64_t rows_stride, size_t num_rows,
+                     const int32_t* positions, const void* weights, const void* grad_out,
+                     uint64_t grad_out_stride, void* grad_rows, uint64_t grad_rows_stride,
+                     void* grad_weights, cudaStream_t s) {
+  const size_t places = r.n * r.slots;
+  combine_backward_kernel<T, W, kVec, kLanes>
+      <<<blocks_for(places * kLanes), kRowThreads, 0, counted(s)>>>(
+          static_cast<uint32_t>(places), FastDiv(static_cast<uint32_t>(r.slots)),
+          static_cast<uint32_t>(r.dim / kVec), static_cast<const T*>(rows), rows_stride,
+          static_cast<uint32_t>(num_rows), positions, static_cast<const W*>(weights),
+          static_cast<const T*>(grad_out), grad_out_stride, static_cast<T*>(grad_rows),
+          grad_rows_stride, static_cast<W*>(grad_weights));
+  CUDA_TRY(cudaGetLastError());
+}
+
+// calls f with the row type and the weight type as values of those types
+template <class F>
+void with_types(int value_type, int weight_type, F f) {
+  auto pick = [&](auto t) {
+    if (weight_type == value_type)
+      f(t, t);
+    else
+      f(t, float{});
+  };
+  if (value_type == HKV_VALUE_F32)
+    f(float{}, float{});
+  else if (value_type == HKV_VALUE_F16)
+    pick(__half{});
+  else
+    pick(__nv_bfloat16{});
+}
+
+int check_combine_types(int value_type, const void* weights, const void* grad_weights,
+                        int weight_type) {
+  HKV_REQUIRE(value_type == HKV_VALUE_F32 || value_type == HKV_VALUE_F16 ||
+                  value_type == HKV_VALUE_BF16,
+              HKV_ERR_UNSUPPORTED, "rows to combine are float32, float16 or bfloat16");
+  if (weights == nullptr && grad_weights == nullptr) return value_type;
+  HKV_REQUIRE(weight_type == HKV_VALUE_F32 || weight_type == value_type, HKV_ERR_INVALID,
+              "weights are float32 or of the rows' type");
+  return weight_type;
+}
+
+}  // namespace
+}  // namespace hkvb
+
+// ===========================================================================
+// C ABI
+// ===========================================================================
+using hkvb::HkvError;
+
+#define HKV_API_BEGIN try {
+#define HKV_API_END                     \
+  return HKV_OK;                        \
+  }                                     \
+  catch (const HkvError& e) {           \
+    hkvb::set_last_error(e.msg);        \
+    return e.code;                      \
+  }                                     \
+  catch (const std::exception& e) {     \
+    hkvb::set_last_error(e.what());     \
+    return HKV_ERR_RUNTIME;             \
+  }
+
+extern "C" {
+
+int hkv_group_workspace(size_t n, uint32_t num_groups, size_t* out_bytes) {
+  HKV_API_BEGIN
+  HKV_REQUIRE(out_bytes != nullptr, HKV_ERR_INVALID, "null argument");
+  HKV_REQUIRE(n <= hkvb::kMaxCount, HKV_ERR_INVALID, "n must be below 2^31");
+  HKV_REQUIRE(num_groups > 0 && num_groups <= HKV_MAX_GROUPS, HKV_ERR_INVALID,
+              "num_groups must be 1 to 4096");
+  *out_bytes = hkvb::sort_workspace(n, num_groups);
+  HKV_API_END
+}
+
+int hkv_group_tokens(size_t n, const void* groups, int id_type, uint32_t num_groups,
+                     int32_t* offsets, int32_t* positions, int32_t* order, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  HKV_API_BEGIN
+  HKV_REQUIRE(id_type == HKV_ID_I32 || id_type == HKV_ID_I64, HKV_ERR_INVALID,
+              "unknown id type");
+  HKV_REQUIRE(n <= hkvb::kMaxCount, HKV_ERR_INVALID, "n must be below 2^31");
+  HKV_REQUIRE(num_groups > 0 && num_groups <= HKV_MAX_GROUPS, HKV_ERR_INVALID,
+              "num_groups must be 1 to 4096");
+  hkvb::require(offsets, 4, "offsets");
+  if (n > 0) {
+    hkvb::require(groups, id_type == HKV_ID_I32 ? 4 : 8, "groups");
+    hkvb::require(positions, 4, "positions");
+    if (order) hkvb::require(order, 4, "order");
+  }
+  hkvb::require(workspace, 16, "workspace");
+  HKV_REQUIRE(workspace_bytes >= hkvb::sort_workspace(n, num_groups), HKV_ERR_INVALID,
+              "the workspace is smaller than hkv_group_workspace asks for");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (id_type == HKV_ID_I32)
+    hkvb::launch_sort<int32_t>(n, groups, num_groups, offsets, positions, order, workspace, s);
+  else
+    hkvb::launch_sort<int64_t>(n, groups, num_groups, offsets, positions, order, workspace, s);
+  HKV_API_END
+}
+
+int hkv_dispatch_rows(size_t n, size_t slots, size_t dim, int value_type, const void* x,
+                      size_t x_stride, const int32_t* positions, size_t num_rows, void* rows,
+                      size_t rows_stride, void* stream) {
+  HKV_API_BEGIN
+  const hkvb::RowShape r = hkvb::check_shape(n, slots, dim, value_type, num_rows);
+  const uint64_t xs = hkvb::stride_or(x_stride, dim, "x_stride");
+  const uint64_t rs = hkvb::stride_or(rows_stride, dim, "rows_stride");
+  if (n == 0 || num_rows == 0) return HKV_OK;
+  hkvb::require(x, r.bytes, "x");
+  hkvb::require(positions, 4, "positions");
+  hkvb::require(rows, r.bytes, "rows");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (hkvb::word_bytes({x, rows}, {dim * r.bytes, xs * r.bytes, rs * r.bytes})) {
+    case 16: hkvb::launch_dispatch<16>(r, x, xs, positions, num_rows, rows, rs, s); break;
+    case 8: hkvb::launch_dispatch<8>(r, x, xs, positions, num_rows, rows, rs, s); break;
+    case 4: hkvb::launch_dispatch<4>(r, x, xs, positions, num_rows, rows, rs, s); break;
+    case 2: hkvb::launch_dispatch<2>(r, x, xs, positions, num_rows, rows, rs, s); break;
+    default: hkvb::launch_dispatch<1>(r, x, xs, positions, num_rows, rows, rs, s);
+  }
+  HKV_API_END
+}
+
+int hkv_combine_rows(size_t n, size_t slots, size_t dim, int value_type, const void* rows,
+                     size_t rows_stride, size_t num_rows, const int32_t* positions,
+                     const void* weights, int weight_type, void* out, size_t out_stride,
+                     void* stream) {
+  HKV_API_BEGIN
+  const hkvb::RowShape r = hkvb::check_shape(n, slots, dim, value_type, num_rows);
+  const int wt = hkvb::check_combine_types(value_type, weights, nullptr, weight_type);
+  const uint64_t rs = hkvb::stride_or(rows_stride, dim, "rows_stride");
+  const uint64_t os = hkvb::stride_or(out_stride, dim, "out_stride");
+  if (n == 0) return HKV_OK;
+  if (num_rows > 0) hkvb::require(rows, r.bytes, "rows");
+  if (positions) hkvb::require(positions, 4, "positions");
+  if (weights) hkvb::require(weights, hkvb::type_bytes(wt), "weights");
+  hkvb::require(out, r.bytes, "out");
+  const bool wide =
+      hkvb::word_bytes({rows, out}, {dim * r.bytes, rs * r.bytes, os * r.bytes}) == 16;
+  hkvb::with_types(value_type, wt, [&](auto t, auto w) {
+    using T = decltype(t);
+    using W = decltype(w);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (wide)
+      hkvb::launch_combine<T, W, 16 / sizeof(T)>(r, rows, rs, num_rows, positions, weights, out,
+                                                 os, s);
+    else
+      hkvb::launch_combine<T, W, 1>(r, rows, rs, num_rows, positions, weights, out, os, s);
+  });
+  HKV_API_END
+}
+
+int hkv_combine_rows_backward(size_t n, size_t slots, size_t dim, int value_type,
+                              const void* rows, size_t rows_stride, size_t num_rows,
+                              const int32_t* positions, const void* weights, int weight_type,
+                              const void* grad_out, size_t grad_out_stride, void* grad_rows,
+                              size_t grad_rows_stride, void* grad_weights, void* stream) {
+  HKV_API_BEGIN
+  const hkvb::RowShape r = hkvb::check_shape(n, slots, dim, value_type, num_rows);
+  const int wt = hkvb::check_combine_types(value_type, weights, grad_weights, weight_type);
+  const uint64_t rs = hkvb::stride_or(rows_stride, dim, "rows_stride");
+  const uint64_t gs = hkvb::stride_or(grad_out_stride, dim, "grad_out_stride");
+  const uint64_t ys = hkvb::stride_or(grad_rows_stride, dim, "grad_rows_stride");
+  if (n == 0 || (grad_rows == nullptr && grad_weights == nullptr)) return HKV_OK;
+  hkvb::require(grad_out, r.bytes, "grad_out");
+  if (positions) hkvb::require(positions, 4, "positions");
+  if (weights) hkvb::require(weights, hkvb::type_bytes(wt), "weights");
+  if (grad_rows) hkvb::require(grad_rows, r.bytes, "grad_rows");
+  if (grad_weights) {
+    if (num_rows > 0) hkvb::require(rows, r.bytes, "rows");
+    hkvb::require(grad_weights, hkvb::type_bytes(wt), "grad_weights");
+  }
+  const bool wide = hkvb::word_bytes({grad_weights ? rows : nullptr, grad_out, grad_rows},
+                                     {dim * r.bytes, rs * r.bytes, gs * r.bytes,
+                                      ys * r.bytes}) == 16;
+  hkvb::with_types(value_type, wt, [&](auto t, auto w) {
+    using T = decltype(t);
+    using W = decltype(w);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    auto go = [&](auto vec, auto lanes) {
+      hkvb::launch_backward<T, W, decltype(vec)::value, decltype(lanes)::value>(
+          r, rows, rs, num_rows, positions, weights, grad_out, gs, grad_rows, ys, grad_weights,
+          s);
+    };
+    auto pick = [&](auto vec) {
+      const size_t packs = dim / decltype(vec)::value;
+      if (packs <= 8)
+        go(vec, std::integral_constant<int, 8>{});
+      else
+        go(vec, std::integral_constant<int, 32>{});
+    };
+    if (wide)
+      pick(std::integral_constant<int, 16 / sizeof(T)>{});
+    else
+      pick(std::integral_constant<int, 1>{});
+  });
+  HKV_API_END
+}
+
+}  // extern "C"

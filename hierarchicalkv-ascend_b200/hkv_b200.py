@@ -145,6 +145,24 @@ class _Allocator(ctypes.Structure):
 
 MEMORY_DEVICE, MEMORY_PINNED, MEMORY_HOST = 0, 1, 2
 
+
+class _PagesOptions(ctypes.Structure):
+    _fields_ = [
+        ("num_pages", ctypes.c_uint32),
+        ("page_tokens", ctypes.c_uint32),
+        ("num_rows", ctypes.c_uint32),
+        ("max_pages", ctypes.c_uint32),
+        ("table_stride", ctypes.c_uint64),
+        ("refs", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("num_planes", ctypes.c_uint32),
+        ("device_id", ctypes.c_int),
+        ("planes", ctypes.POINTER(ctypes.c_void_p)),
+        ("page_bytes", ctypes.POINTER(ctypes.c_uint64)),
+    ]
+
+
 # C ABI symbols and their signatures (include/hkv_b200.h)
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
@@ -214,6 +232,24 @@ SIGNATURES = {
     "hkv_sharded_find": (ctypes.c_int, [_P, _SZ, _P, _P, _P, _P, _P]),
     "hkv_sharded_insert_or_assign": (ctypes.c_int, [_P, _SZ, _P, _P, _P, _P, _B]),
     "hkv_sharded_size": (ctypes.c_int, [_P, _P, ctypes.POINTER(_SZ)]),
+    "hkv_group_workspace": (ctypes.c_int, [_SZ, ctypes.c_uint32, ctypes.POINTER(_SZ)]),
+    "hkv_group_tokens": (ctypes.c_int, [_SZ, _P, ctypes.c_int, ctypes.c_uint32, _P, _P, _P,
+                                        _P, _SZ, _P]),
+    "hkv_dispatch_rows": (ctypes.c_int, [_SZ, _SZ, _SZ, ctypes.c_int, _P, _SZ, _P, _SZ, _P,
+                                         _SZ, _P]),
+    "hkv_combine_rows": (ctypes.c_int, [_SZ, _SZ, _SZ, ctypes.c_int, _P, _SZ, _SZ, _P, _P,
+                                        ctypes.c_int, _P, _SZ, _P]),
+    "hkv_combine_rows_backward": (ctypes.c_int, [_SZ, _SZ, _SZ, ctypes.c_int, _P, _SZ, _SZ, _P,
+                                                 _P, ctypes.c_int, _P, _SZ, _P, _SZ, _P, _P]),
+    "hkv_pages_create": (ctypes.c_int, [ctypes.POINTER(_PagesOptions),
+                                        ctypes.POINTER(_Allocator), ctypes.POINTER(_P)]),
+    "hkv_pages_destroy": (ctypes.c_int, [_P]),
+    "hkv_pages_copy": (ctypes.c_int, [_P, _SZ, _P, _P, _P]),
+    "hkv_pages_fork": (ctypes.c_int, [_P, _SZ, _P, _P, _P]),
+    "hkv_pages_resize": (ctypes.c_int, [_P, _SZ, _P, _P, _P, _P]),
+    "hkv_pages_free": (ctypes.c_int, [_P, _SZ, _P, _P]),
+    "hkv_pages_hold": (ctypes.c_int, [_P, _SZ, _P, ctypes.c_int, _P]),
+    "hkv_pages_compact": (ctypes.c_int, [_P, _P, _P, _P, _P]),
 }
 
 
@@ -737,3 +773,411 @@ class ShardedHashTable:
         out = ctypes.c_size_t(0)
         _check(lib().hkv_sharded_size(self._h, _stream(stream), ctypes.byref(out)))
         return out.value
+
+
+# ---- tokens sorted by group, and back (no reference counterpart) ------------
+# Functions on torch CUDA tensors with caller-allocated outputs, as the table's
+# methods; n tokens at the front of each tensor take part, what lies behind them
+# stays as it was. They run on the tensors' device and, unless told otherwise,
+# on its current stream.
+
+_IDS = _ROW_TYPES = None
+
+
+def _row_types():
+    """(value type by torch dtype, id type by torch dtype)"""
+    global _IDS, _ROW_TYPES
+    if _ROW_TYPES is None:
+        import torch as t
+
+        _IDS = {t.int32: 0, t.int64: 1}
+        _ROW_TYPES = {t.float32: 0, t.float16: 1, t.bfloat16: 2, t.float64: 3, t.int32: 4,
+                      t.uint32: 4, t.int16: 5, t.uint16: 5, t.int8: 6, t.uint8: 6, t.int64: 7,
+                      t.uint64: 7}
+    return _ROW_TYPES, _IDS
+
+
+def _refuse_unless(ok, message):
+    if not ok:
+        raise HkvException(message)
+
+
+def _matrix(t, name, n=0):
+    """(rows, dim, elements from row to row) of a 2-D tensor whose rows are
+    contiguous and do not overlap."""
+    _refuse_unless(t.dim() == 2, f"{name} must have two dimensions")
+    rows, dim = t.shape
+    _refuse_unless(n <= rows, f"{name} has {rows} rows, fewer than {n}")
+    _refuse_unless(dim > 0, f"{name} has empty rows")
+    stride, step = t.stride()
+    _refuse_unless(step == 1 or dim == 1, f"the rows of {name} must be contiguous")
+    if rows > 1:
+        _refuse_unless(stride >= dim, f"the rows of {name} overlap (an expanded tensor?)")
+    else:
+        stride = dim
+    return rows, dim, stride
+
+
+def _list(t, name, n, dtype):
+    """A contiguous tensor of at least n elements of one dtype."""
+    _refuse_unless(t.dtype == dtype, f"{name} must be {dtype}, not {t.dtype}")
+    _refuse_unless(t.numel() >= n, f"{name} has {t.numel()} elements, fewer than {n}")
+    _refuse_unless(t.is_contiguous(), f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _one_device(tensors):
+    device = tensors[0].device
+    for t in tensors:
+        _refuse_unless(t.device == device, "the tensors are on different devices")
+    _refuse_unless(device.type == "cuda", "the tensors must be on a CUDA device")
+    return device
+
+
+def _call_on(device, stream, fn, *args):
+    """fn(*args, stream) with the device current."""
+    import torch
+
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    if torch.cuda.current_device() == device.index:
+        _check(fn(*args, _stream(stream)))
+    else:
+        with torch.cuda.device(device):
+            _check(fn(*args, _stream(stream)))
+
+
+def group_workspace(n: int, num_groups: int) -> int:
+    """Bytes of scratch that group_tokens needs for n places."""
+    _refuse_unless(n >= 0 and num_groups >= 0, "n and num_groups must not be negative")
+    _refuse_unless(num_groups < 1 << 32, "num_groups must be 1 to 4096")
+    out = _SZ(0)
+    _check(lib().hkv_group_workspace(n, num_groups, ctypes.byref(out)))
+    return out.value
+
+
+def group_tokens(n, groups, num_groups, offsets, positions, order=None, workspace=None,
+                 stream=None):
+    """Sorts n places (n tokens times their slots) by their group, keeping the
+    order of places of one group. groups: int32 or int64; positions (int32)
+    receives the row of each place, order (int32, optional) the place of each
+    row, offsets (int32, num_groups + 1) the first row of each group. A place
+    whose group is outside [0, num_groups) gets the position -1. workspace: a
+    uint8 tensor of group_workspace(n, num_groups) bytes, allocated here when
+    None; calls that may overlap need their own."""
+    import torch
+
+    _refuse_unless(n >= 0, "n must not be negative")
+    ids = _row_types()[1].get(groups.dtype)
+    _refuse_unless(ids is not None, f"groups must be int32 or int64, not {groups.dtype}")
+    g = _list(groups, "groups", n, groups.dtype)
+    p = _list(positions, "positions", n, torch.int32)
+    f = _list(offsets, "offsets", num_groups + 1, torch.int32)
+    tensors = [groups, positions, offsets]
+    r = None
+    if order is not None:
+        r = _list(order, "order", n, torch.int32)
+        tensors.append(order)
+    size = group_workspace(n, num_groups) if workspace is None else 0
+    if workspace is not None:
+        size = workspace.numel() * workspace.element_size()
+        _refuse_unless(workspace.is_contiguous(), "workspace must be contiguous")
+        tensors.append(workspace)
+    device = _one_device(tensors)
+    if workspace is None:
+        if isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream, device)
+        # from the pool of the stream that uses it
+        with torch.cuda.stream(stream or torch.cuda.current_stream(device)):
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    _call_on(device, stream, lib().hkv_group_tokens, n, g, ids, num_groups, f, p, r,
+             workspace.data_ptr(), size)
+
+
+def _positions(n, positions):
+    """(address, slots) of the int32 positions [tokens, slots]."""
+    import torch
+
+    _refuse_unless(positions.dim() == 2 and positions.shape[1] > 0,
+                   "positions must be [tokens, slots]")
+    _refuse_unless(n <= positions.shape[0],
+                   f"positions has {positions.shape[0]} tokens, fewer than {n}")
+    return _list(positions, "positions", 0, torch.int32), positions.shape[1]
+
+
+def dispatch_rows(n, x, positions, rows, stream=None):
+    """rows[positions[t, s]] = x[t] for the first n tokens, any value type.
+    x: [tokens, dim], positions: int32 [tokens, slots], rows: [rows, dim]; a
+    position outside rows is passed over and rows that no place has stay as
+    they were. The gradient: combine_rows(n, grad_rows, positions, None, grad_x)."""
+    _refuse_unless(n >= 0, "n must not be negative")
+    _, dim, x_stride = _matrix(x, "x", n)
+    num_rows, width, rows_stride = _matrix(rows, "rows")
+    _refuse_unless(width == dim and rows.dtype == x.dtype, "x and rows differ in dim or type")
+    kind = _row_types()[0].get(x.dtype)
+    _refuse_unless(kind is not None, f"rows of {x.dtype} are not supported")
+    p, slots = _positions(n, positions)
+    device = _one_device((x, positions, rows))
+    _call_on(device, stream, lib().hkv_dispatch_rows, n, slots, dim, kind, x.data_ptr(),
+             x_stride, p, num_rows, rows.data_ptr(), rows_stride)
+
+
+def _weights(weights, name, n, slots, kind):
+    _refuse_unless(weights.dim() == 2 and weights.shape[1] == slots and weights.shape[0] >= n,
+                   f"{name} must be [tokens, slots]")
+    _refuse_unless(weights.is_contiguous(), f"{name} must be contiguous")
+    got = _row_types()[0].get(weights.dtype)
+    _refuse_unless(got in (0, kind), f"{name} must be float32 or of the rows' type")
+    return got
+
+
+def _by_place(slots, *shaped):
+    """Slots of a call without positions: as told, else those of the weights."""
+    for t in shaped:
+        if t is not None and slots is None:
+            slots = t.shape[-1]
+    _refuse_unless(slots is not None and slots > 0,
+                   "without positions and weights, slots must be given")
+    return slots
+
+
+def combine_rows(n, rows, positions, weights, out, stream=None, slots=None):
+    """out[t] = sum over s of weights[t, s] * rows[positions[t, s]] for the
+    first n tokens. rows: [rows, dim] of float32, float16 or bfloat16;
+    weights: [tokens, slots] of float32 or the rows' type, None for ones;
+    out: [tokens, dim]. positions None: the row of place (t, s) is t * slots +
+    s (what find wrote for the keys of n tokens), with slots as given or those
+    of weights. Summed in float32, rounded once."""
+    _refuse_unless(n >= 0, "n must not be negative")
+    num_rows, dim, rows_stride = _matrix(rows, "rows")
+    _, width, out_stride = _matrix(out, "out", n)
+    _refuse_unless(width == dim and rows.dtype == out.dtype, "rows and out differ in dim or type")
+    kind = _row_types()[0].get(rows.dtype)
+    _refuse_unless(kind is not None, f"rows of {rows.dtype} are not supported")
+    tensors = [rows, out]
+    if positions is not None:
+        p, slots = _positions(n, positions)
+        tensors.append(positions)
+    else:
+        p, slots = None, _by_place(slots, weights)
+    w = w_kind = None
+    if weights is not None:
+        w_kind = _weights(weights, "weights", n, slots, kind)
+        w = weights.data_ptr()
+        tensors.append(weights)
+    device = _one_device(tensors)
+    _call_on(device, stream, lib().hkv_combine_rows, n, slots, dim, kind, rows.data_ptr(),
+             rows_stride, num_rows, p, w, w_kind or 0, out.data_ptr(), out_stride)
+
+
+def combine_rows_backward(n, rows, positions, weights, grad_out, grad_rows=None,
+                          grad_weights=None, stream=None, slots=None):
+    """Gradients of combine_rows: grad_rows[positions[t, s]] = weights[t, s] *
+    grad_out[t] (rows without a place stay as they were) and grad_weights[t, s]
+    = the inner product of grad_out[t] and rows[positions[t, s]] (0 for a place
+    without a row), either left out when None. Each row may be the row of one
+    place only. rows may be None when grad_weights is. Without positions, slots
+    as given or those of weights or grad_weights."""
+    _refuse_unless(n >= 0, "n must not be negative")
+    _, dim, out_stride = _matrix(grad_out, "grad_out", n)
+    kind = _row_types()[0].get(grad_out.dtype)
+    _refuse_unless(kind is not None, f"rows of {grad_out.dtype} are not supported")
+    _refuse_unless(rows is not None or grad_weights is None, "grad_weights needs rows")
+    if grad_rows is None and grad_weights is None:
+        return
+    tensors, num_rows, rows_stride, grad_stride = [grad_out], None, 0, 0
+    for t, name in ((rows, "rows"), (grad_rows, "grad_rows")):
+        if t is None:
+            continue
+        count, width, stride = _matrix(t, name)
+        _refuse_unless(width == dim and t.dtype == grad_out.dtype,
+                       f"{name} and grad_out differ in dim or type")
+        _refuse_unless(num_rows in (None, count), "rows and grad_rows differ in rows")
+        num_rows = count
+        if name == "rows":
+            rows_stride = stride
+        else:
+            grad_stride = stride
+        tensors.append(t)
+    if positions is not None:
+        p, slots = _positions(n, positions)
+        tensors.append(positions)
+    else:
+        p, slots = None, _by_place(slots, weights, grad_weights)
+    w_kind = 0
+    for t, name in ((weights, "weights"), (grad_weights, "grad_weights")):
+        if t is not None:
+            w_kind = _weights(t, name, n, slots, kind)
+            tensors.append(t)
+    if weights is not None and grad_weights is not None:
+        _refuse_unless(weights.dtype == grad_weights.dtype,
+                       "weights and grad_weights differ in type")
+    device = _one_device(tensors)
+    _call_on(device, stream, lib().hkv_combine_rows_backward, n, slots, dim, kind, _ptr(rows),
+             rows_stride, num_rows, p, _ptr(weights), w_kind, grad_out.data_ptr(), out_stride,
+             _ptr(grad_rows), grad_stride, _ptr(grad_weights))
+
+
+class PagePool:
+    """Pages of a cache whose index is a table (no reference counterpart; see
+    hkv_pages in include/hkv_b200.h for the rules of each call).
+
+    planes: the cache's tensors (for instance keys and values of each layer),
+    each contiguous with the pages as first dimension; page_tokens: tokens of a
+    page. refs (int32 [pages]: 0 is a free page), table (int32 [rows,
+    max_pages]: page numbers of each sequence) and lengths (int32 [rows]:
+    tokens) are the pool's state; they are made here, empty, from num_rows and
+    max_pages unless given. Calls on one pool must be ordered by the caller.
+
+    With a HashTable of page numbers as its index, hold(n, pages, 1) keeps the
+    pages that the index names in use, and hold(n, evicted_values, -1) lets go
+    of those that insert_and_evict gave back (a number out of range, such as
+    -1, is passed over)."""
+
+    def __init__(self, planes, page_tokens, num_rows=None, max_pages=None, num_pages=None,
+                 refs=None, table=None, lengths=None, allocator=None):
+        import torch
+
+        self._h = None
+        planes = list(planes)
+        given = planes + [t for t in (refs, table, lengths) if t is not None]
+        if given:
+            device = given[0].device
+        else:
+            device = torch.device("cuda", torch.cuda.current_device())
+        if num_pages is None:
+            sized = planes[0] if planes else refs
+            _refuse_unless(sized is not None and sized.dim() > 0, "num_pages is not given")
+            num_pages = sized.shape[0]
+        for k, t in enumerate(planes):
+            _refuse_unless(t.dim() > 0 and t.shape[0] == num_pages,
+                           f"plane {k} does not have {num_pages} pages")
+            _refuse_unless(t.is_contiguous(), f"plane {k} must be contiguous")
+            _refuse_unless(t.numel() > 0, f"plane {k} is empty")
+        if table is not None:
+            rows, width, stride = _matrix(table, "table")
+            _refuse_unless(table.dtype == torch.int32, "table must be int32")
+            _refuse_unless(num_rows in (None, rows) and max_pages in (None, width),
+                           "table differs from num_rows or max_pages")
+            num_rows, max_pages = rows, width
+        _refuse_unless(num_rows is not None and max_pages is not None,
+                       "num_rows and max_pages are not given")
+        for name, v in (("num_pages", num_pages), ("page_tokens", page_tokens),
+                        ("num_rows", num_rows), ("max_pages", max_pages)):
+            _refuse_unless(0 < v < 1 << 31, f"{name} must be positive and below 2^31")
+        if refs is not None:
+            _list(refs, "refs", num_pages, torch.int32)
+        if lengths is not None:
+            _list(lengths, "lengths", num_rows, torch.int32)
+        _refuse_unless(device.type == "cuda", "the tensors must be on a CUDA device")
+        for t in given:
+            _refuse_unless(t.device == device, "the tensors are on different devices")
+        if refs is None:
+            refs = torch.zeros(num_pages, dtype=torch.int32, device=device)
+        if table is None:
+            table = torch.full((num_rows, max_pages), -1, dtype=torch.int32, device=device)
+            stride = max_pages
+        if lengths is None:
+            lengths = torch.zeros(num_rows, dtype=torch.int32, device=device)
+        self.planes, self.refs, self.table, self.lengths = planes, refs, table, lengths
+        self.page_tokens, self.num_pages, self.device = page_tokens, num_pages, device
+        self._table_stride = stride
+        o = _PagesOptions(num_pages=num_pages, page_tokens=page_tokens, num_rows=num_rows,
+                          max_pages=max_pages, table_stride=stride, refs=refs.data_ptr(),
+                          table=table.data_ptr(), lengths=lengths.data_ptr(),
+                          num_planes=len(planes), device_id=device.index)
+        o.planes = (_P * max(len(planes), 1))(*[t.data_ptr() for t in planes])
+        o.page_bytes = (_U64 * max(len(planes), 1))(
+            *[t.numel() // num_pages * t.element_size() for t in planes])
+        self._alloc_cbs = None if allocator is None else _allocator_callbacks(allocator)
+        h = ctypes.c_void_p()
+        _check(lib().hkv_pages_create(
+            ctypes.byref(o), None if allocator is None else ctypes.byref(self._alloc_cbs),
+            ctypes.byref(h)))
+        self._h = h.value
+
+    def close(self) -> None:
+        if self._h is not None:
+            _check(lib().hkv_pages_destroy(self._h))
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _on_stream(self, stream):
+        if stream is None:
+            import torch
+
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return _stream(stream)
+
+    def _numbers(self, t, name, n):
+        import torch
+
+        _refuse_unless(0 <= n, "n must not be negative")
+        address = _list(t, name, n, torch.int32)
+        _refuse_unless(t.device == self.device, f"{name} is not on the pool's device")
+        return address
+
+    def copy(self, n, src, dst, stream=None):
+        """Copies page src[i] to page dst[i] in every plane. A destination may
+        not be listed twice, nor be the source of another pair."""
+        _check(lib().hkv_pages_copy(self._h, n, self._numbers(src, "src", n),
+                                    self._numbers(dst, "dst", n), self._on_stream(stream)))
+
+    def fork(self, n, src, dst, stream=None):
+        """Row dst[i] becomes a branch of row src[i]: same length, shared pages.
+        What it held before is given back. Sources are read before any row is
+        written."""
+        _check(lib().hkv_pages_fork(self._h, n, self._numbers(src, "src", n),
+                                    self._numbers(dst, "dst", n), self._on_stream(stream)))
+
+    def resize(self, n, rows, lengths, status=None, stream=None):
+        """Row rows[i] gets the length lengths[i]: takes free pages, lowest
+        number first, copies a shared last page before the row writes behind its
+        old length, or gives pages back. status (bool, optional): whether the
+        entry was served; one that was not leaves its row as it was."""
+        import torch
+
+        s = None
+        if status is not None:
+            s = _list(status, "status", n, torch.bool)
+            _refuse_unless(status.device == self.device, "status is not on the pool's device")
+        _check(lib().hkv_pages_resize(self._h, n, self._numbers(rows, "rows", n),
+                                      self._numbers(lengths, "lengths", n), s,
+                                      self._on_stream(stream)))
+
+    def free(self, n, rows, stream=None):
+        """Rows give their pages back and get length 0."""
+        _check(lib().hkv_pages_free(self._h, n, self._numbers(rows, "rows", n),
+                                    self._on_stream(stream)))
+
+    def hold(self, n, pages, delta=1, stream=None):
+        """Adds delta to the count of each listed page."""
+        _refuse_unless(-(1 << 31) <= delta < 1 << 31, "delta must be a 32-bit number")
+        _check(lib().hkv_pages_hold(self._h, n, self._numbers(pages, "pages", n), delta,
+                                    self._on_stream(stream)))
+
+    def compact(self, page_map=None, table_out=None, refs_out=None, stream=None):
+        """Moves the pages in use to the lowest numbers. page_map (int32
+        [pages]) receives each page's new number, -1 for a free page. With
+        table_out and refs_out (like table and refs) the rewritten state goes
+        there and the old table stays valid for readers; otherwise the pool's own
+        is rewritten."""
+        import torch
+
+        m = t = r = None
+        if page_map is not None:
+            m = self._numbers(page_map, "page_map", self.num_pages)
+        if refs_out is not None:
+            r = self._numbers(refs_out, "refs_out", self.num_pages)
+        if table_out is not None:
+            _refuse_unless(table_out.dtype == torch.int32 and table_out.shape == self.table.shape
+                           and table_out.device == self.device, "table_out is not like table")
+            _refuse_unless(_matrix(table_out, "table_out")[2] == self._table_stride,
+                           "table_out and table differ in stride")
+            t = table_out.data_ptr()
+        _check(lib().hkv_pages_compact(self._h, m, t, r, self._on_stream(stream)))

@@ -473,6 +473,167 @@ int hkv_sharded_insert_or_assign(hkv_sharded* s, size_t n, const void* keys,
 /* Collective sum of the shard sizes. */
 int hkv_sharded_size(hkv_sharded* s, void* stream, size_t* out);
 
+/* ---- tokens sorted by group, and back (no reference counterpart) -----------
+ * A model sends each of its n tokens to `slots` groups: the experts of a
+ * layer, the tables of its features, the owners of its keys. Sorted by group,
+ * the places (token, slot) become rows; what comes out of the groups goes back
+ * to the tokens with weights. Place i = token * slots + slot. All pointers are
+ * memory of the current device; the calls are asynchronous on `stream`,
+ * allocate nothing and can be captured into a graph. Counts of places and rows
+ * stay below 2^31. Outputs must not overlap inputs or one another.
+ *
+ * Rows are `dim` elements of `value_type`, `*_stride` elements apart (at least
+ * dim; 0 means dim). A position outside [0, num_rows) means that the place has
+ * no row: nothing is read or written for it, whatever its weight holds. */
+typedef enum { HKV_ID_I32 = 0, HKV_ID_I64 = 1 } hkv_id_type;
+
+/* Most groups of one hkv_group_tokens call. */
+#define HKV_MAX_GROUPS 4096
+
+/* Bytes of scratch that hkv_group_tokens needs for n places. */
+int hkv_group_workspace(size_t n, uint32_t num_groups, size_t* out_bytes);
+
+/* Stable sort of n places by groups[i] (id_type): positions[i] is the row of
+ * place i, order[r] (nullable) the place of row r, group g has the rows
+ * offsets[g] to offsets[g + 1] (num_groups + 1 entries). Places of one group
+ * keep their order. A place whose group is outside [0, num_groups) has no row:
+ * its position is -1, and order ends in as many -1. `workspace` (16-byte
+ * aligned) is scratch for this call only: two calls that may run at the same
+ * time need two. */
+int hkv_group_tokens(size_t n, const void* groups, int id_type,
+                     uint32_t num_groups, int32_t* offsets, int32_t* positions,
+                     int32_t* order, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* rows[positions[t * slots + s]] = x[t], any value type. Rows that no place
+ * has stay as they were. Two places with the same position leave one of their
+ * tokens' rows, or a mixture. The gradient of x is hkv_combine_rows of the
+ * gradient of the rows without weights. */
+int hkv_dispatch_rows(size_t n, size_t slots, size_t dim, int value_type,
+                      const void* x, size_t x_stride, const int32_t* positions,
+                      size_t num_rows, void* rows, size_t rows_stride,
+                      void* stream);
+
+/* out[t] = sum over s of weights[t * slots + s] * rows[positions[t * slots + s]],
+ * summed in float32 in the order of the slots and rounded once; F32, F16 and
+ * BF16 rows. weights (nullable: ones) are of weight_type, F32 or value_type.
+ * positions NULL: place i has row i (the rows that hkv_find wrote for n *
+ * slots keys). A token without rows gets zeros. */
+int hkv_combine_rows(size_t n, size_t slots, size_t dim, int value_type,
+                     const void* rows, size_t rows_stride, size_t num_rows,
+                     const int32_t* positions, const void* weights,
+                     int weight_type, void* out, size_t out_stride,
+                     void* stream);
+
+/* Gradients of hkv_combine_rows, each of them nullable:
+ * grad_rows[positions[i]] = weights[i] * grad_out[t], rows that no place has
+ * as they were; grad_weights[i] (weight_type) = the inner product of
+ * grad_out[t] and rows[positions[i]], summed in float32 in an order that
+ * depends on the sizes only, 0 for a place without a row. Every row is the
+ * row of one place at most, as hkv_group_tokens makes them; a row of several
+ * places would get the gradient of one of them, or a mixture. rows is read
+ * for grad_weights only. */
+int hkv_combine_rows_backward(size_t n, size_t slots, size_t dim,
+                              int value_type, const void* rows,
+                              size_t rows_stride, size_t num_rows,
+                              const int32_t* positions, const void* weights,
+                              int weight_type, const void* grad_out,
+                              size_t grad_out_stride, void* grad_rows,
+                              size_t grad_rows_stride, void* grad_weights,
+                              void* stream);
+
+/* ---- pages of a cache (no reference counterpart) ----------------------------
+ * A model's cache of past tokens in pages, for programs that keep a table as
+ * its index (key: hash of a block of tokens; value: page number; the values
+ * that insert_and_evict gives back are pages to let go). The caller owns the
+ * memory: planes (for instance keys and values of each layer; page p of plane
+ * k is page_bytes[k] bytes at planes[k] + p * page_bytes[k]), one reference
+ * count per page (0: free), and a page table with a length in tokens per row
+ * (sequence). A row of length L holds the pages table[row][0 .. ceil(L /
+ * page_tokens)); entries behind them mean nothing and stay as they were. Rows
+ * may share pages; a count is the number of rows that hold the page, plus
+ * what hkv_pages_hold added.
+ *
+ * All calls are asynchronous on `stream`, run on the pool's device whichever
+ * is current, allocate nothing and can be captured into a graph; they share
+ * the pool's scratch, so calls on one pool must be ordered by the caller
+ * (one stream, or events). Lists of rows and pages are device memory; a row
+ * or page number out of range is passed over, in lists and in the table. */
+typedef struct hkv_pages hkv_pages;
+
+#define HKV_MAX_PLANES 128
+
+typedef struct {
+  uint32_t num_pages;
+  uint32_t page_tokens;  /* tokens per page */
+  uint32_t num_rows;     /* rows of the page table */
+  uint32_t max_pages;    /* pages of a row at most; max_pages * page_tokens < 2^31 */
+  uint64_t table_stride; /* entries from row to row, 0 means max_pages */
+  int32_t* refs;         /* num_pages counts, 16-byte aligned */
+  int32_t* table;        /* num_rows rows */
+  int32_t* lengths;      /* num_rows */
+  uint32_t num_planes;   /* 0 to HKV_MAX_PLANES */
+  int device_id;         /* -1: current device */
+  void* const* planes;        /* host array of num_planes device addresses */
+  const uint64_t* page_bytes; /* host array of num_planes sizes */
+} hkv_pages_options;
+
+/* The caller's arrays are neither read nor changed here (zero refs and
+ * lengths for an empty cache) and must outlive the pool; scratch comes from
+ * `allocator` (nullable: the CUDA runtime). */
+int hkv_pages_create(const hkv_pages_options* options,
+                     const hkv_allocator* allocator, hkv_pages** out);
+/* Waits for the pool's device. */
+int hkv_pages_destroy(hkv_pages* pool);
+
+/* Copies page src[i] to page dst[i] in every plane. As with memcpy, a page may
+ * be the destination of one pair only, and then not the source of another:
+ * the content of such a page is not defined. */
+int hkv_pages_copy(hkv_pages* pool, size_t n, const int32_t* src,
+                   const int32_t* dst, void* stream);
+
+/* Row dst[i] becomes row src[i]: it takes the length and shares the pages
+ * (counts + 1), and the pages that it held before are given back (counts - 1).
+ * Every source is read before any row is written, so beams can be permuted in
+ * place. Of entries with the same dst the last one counts. n is at most
+ * num_rows. */
+int hkv_pages_fork(hkv_pages* pool, size_t n, const int32_t* src,
+                   const int32_t* dst, void* stream);
+
+/* Row rows[i] gets the length lengths[i] (tokens). Growing takes free pages;
+ * where its last page is only partly filled and shared, the row first gets a
+ * copy of that page, so that what is written behind the old length is seen by
+ * this row alone. Shrinking gives pages back. Free pages are those that are
+ * free as the call begins; they are handed out lowest number first, to the
+ * entries in their order (an entry's copy first, then its new pages).
+ * status[i] (nullable) tells whether the entry was served. One that was not
+ * leaves its row as it was: its length is negative or needs more than
+ * max_pages, or it needs pages and all entries up to and with it want more
+ * than are free, or its row comes again later in the list (the last one
+ * counts) or does not exist. n is at most num_rows. */
+int hkv_pages_resize(hkv_pages* pool, size_t n, const int32_t* rows,
+                     const int32_t* lengths, bool* status, void* stream);
+
+/* Rows give their pages back and get length 0. A row may be listed twice. */
+int hkv_pages_free(hkv_pages* pool, size_t n, const int32_t* rows,
+                   void* stream);
+
+/* Adds delta to the count of each listed page (a page listed twice counts
+ * twice): +1 for a page that an index now names, -1 for one that it lets go. */
+int hkv_pages_hold(hkv_pages* pool, size_t n, const int32_t* pages, int delta,
+                   void* stream);
+
+/* Moves the pages in use to the numbers 0 to their number - 1: those already
+ * there stay, the others fill the free ones, both in rising order. page_map
+ * (nullable, num_pages) gets each page's new number, -1 for a free page.
+ * table_out (table_stride apart) and refs_out receive the rewritten page table
+ * and counts; NULL rewrites the pool's own. No page in use is overwritten, so
+ * with both given, readers of the old table go on seeing their tokens until
+ * the new one is put in its place and pages are taken from it. A table entry
+ * whose page is free or out of range becomes -1. */
+int hkv_pages_compact(hkv_pages* pool, int32_t* page_map, int32_t* table_out,
+                      int32_t* refs_out, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
