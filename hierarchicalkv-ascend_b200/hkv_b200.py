@@ -781,20 +781,33 @@ class ShardedHashTable:
 # stays as it was. They run on the tensors' device and, unless told otherwise,
 # on its current stream.
 
-_IDS = _ROW_TYPES = None
+class _Torch:
+    """What the calls below need of torch, looked up once: a call's checks are a
+    large part of its time where it moves few rows."""
 
-
-def _row_types():
-    """(value type by torch dtype, id type by torch dtype)"""
-    global _IDS, _ROW_TYPES
-    if _ROW_TYPES is None:
+    def __init__(self):
         import torch as t
 
-        _IDS = {t.int32: 0, t.int64: 1}
-        _ROW_TYPES = {t.float32: 0, t.float16: 1, t.bfloat16: 2, t.float64: 3, t.int32: 4,
-                      t.uint32: 4, t.int16: 5, t.uint16: 5, t.int8: 6, t.uint8: 6, t.int64: 7,
-                      t.uint64: 7}
-    return _ROW_TYPES, _IDS
+        self.torch = t
+        self.int32, self.bool = t.int32, t.bool
+        self.ids = {t.int32: 0, t.int64: 1}
+        self.rows = {t.float32: 0, t.float16: 1, t.bfloat16: 2, t.float64: 3, t.int32: 4,
+                     t.uint32: 4, t.int16: 5, t.uint16: 5, t.int8: 6, t.uint8: 6, t.int64: 7,
+                     t.uint64: 7}
+        # the raw handle alone, without a Stream object
+        self.stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: t.cuda.current_stream(index).cuda_stream)
+        self.device = getattr(t._C, "_cuda_getDevice", None) or t.cuda.current_device
+
+
+_TORCH = None
+
+
+def _torch():
+    global _TORCH
+    if _TORCH is None:
+        _TORCH = _Torch()
+    return _TORCH
 
 
 def _refuse_unless(ok, message):
@@ -805,46 +818,47 @@ def _refuse_unless(ok, message):
 def _matrix(t, name, n=0):
     """(rows, dim, elements from row to row) of a 2-D tensor whose rows are
     contiguous and do not overlap."""
-    _refuse_unless(t.dim() == 2, f"{name} must have two dimensions")
-    rows, dim = t.shape
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 2:
+        rows, dim = shape
+        if n <= rows and stride[0] >= dim > 0 and stride[1] == 1:
+            return rows, dim, stride[0]
+    _refuse_unless(len(shape) == 2, f"{name} must have two dimensions")
     _refuse_unless(n <= rows, f"{name} has {rows} rows, fewer than {n}")
     _refuse_unless(dim > 0, f"{name} has empty rows")
-    stride, step = t.stride()
-    _refuse_unless(step == 1 or dim == 1, f"the rows of {name} must be contiguous")
-    if rows > 1:
-        _refuse_unless(stride >= dim, f"the rows of {name} overlap (an expanded tensor?)")
-    else:
-        stride = dim
-    return rows, dim, stride
+    _refuse_unless(stride[1] == 1 or dim == 1, f"the rows of {name} must be contiguous")
+    _refuse_unless(stride[0] >= dim or rows <= 1,
+                   f"the rows of {name} overlap (an expanded tensor?)")
+    return rows, dim, max(stride[0], dim)
 
 
 def _list(t, name, n, dtype):
     """A contiguous tensor of at least n elements of one dtype."""
+    if t.dtype is dtype and t.numel() >= n and t.is_contiguous():
+        return t.data_ptr()
     _refuse_unless(t.dtype == dtype, f"{name} must be {dtype}, not {t.dtype}")
     _refuse_unless(t.numel() >= n, f"{name} has {t.numel()} elements, fewer than {n}")
-    _refuse_unless(t.is_contiguous(), f"{name} must be contiguous")
-    return t.data_ptr()
+    raise HkvException(f"{name} must be contiguous")
 
 
 def _one_device(tensors):
-    device = tensors[0].device
+    """Index of the CUDA device that all the tensors are on."""
+    index = tensors[0].get_device()
+    _refuse_unless(index >= 0, "the tensors must be on a CUDA device")
     for t in tensors:
-        _refuse_unless(t.device == device, "the tensors are on different devices")
-    _refuse_unless(device.type == "cuda", "the tensors must be on a CUDA device")
-    return device
+        _refuse_unless(t.get_device() == index, "the tensors are on different devices")
+    return index
 
 
-def _call_on(device, stream, fn, *args):
-    """fn(*args, stream) with the device current."""
-    import torch
-
-    if stream is None:
-        stream = torch.cuda.current_stream(device)
-    if torch.cuda.current_device() == device.index:
-        _check(fn(*args, _stream(stream)))
+def _call_on(index, stream, fn, *args):
+    """fn(*args, stream) with device `index` current."""
+    t = _torch()
+    stream = t.stream(index) if stream is None else _stream(stream)
+    if t.device() == index:
+        _check(fn(*args, stream))
     else:
-        with torch.cuda.device(device):
-            _check(fn(*args, _stream(stream)))
+        with t.torch.cuda.device(index):
+            _check(fn(*args, stream))
 
 
 def group_workspace(n: int, num_groups: int) -> int:
@@ -865,11 +879,11 @@ def group_tokens(n, groups, num_groups, offsets, positions, order=None, workspac
     whose group is outside [0, num_groups) gets the position -1. workspace: a
     uint8 tensor of group_workspace(n, num_groups) bytes, allocated here when
     None; calls that may overlap need their own."""
-    import torch
-
+    torch = _torch()
     _refuse_unless(n >= 0, "n must not be negative")
-    ids = _row_types()[1].get(groups.dtype)
-    _refuse_unless(ids is not None, f"groups must be int32 or int64, not {groups.dtype}")
+    ids = torch.ids.get(groups.dtype)
+    if ids is None:
+        raise HkvException(f"groups must be int32 or int64, not {groups.dtype}")
     g = _list(groups, "groups", n, groups.dtype)
     p = _list(positions, "positions", n, torch.int32)
     f = _list(offsets, "offsets", num_groups + 1, torch.int32)
@@ -880,29 +894,28 @@ def group_tokens(n, groups, num_groups, offsets, positions, order=None, workspac
         tensors.append(order)
     size = group_workspace(n, num_groups) if workspace is None else 0
     if workspace is not None:
-        size = workspace.numel() * workspace.element_size()
+        size = workspace.nbytes
         _refuse_unless(workspace.is_contiguous(), "workspace must be contiguous")
         tensors.append(workspace)
-    device = _one_device(tensors)
+    index = _one_device(tensors)
     if workspace is None:
+        cuda = torch.torch.cuda
         if isinstance(stream, int):
-            stream = torch.cuda.ExternalStream(stream, device)
+            stream = cuda.ExternalStream(stream, index)
         # from the pool of the stream that uses it
-        with torch.cuda.stream(stream or torch.cuda.current_stream(device)):
-            workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    _call_on(device, stream, lib().hkv_group_tokens, n, g, ids, num_groups, f, p, r,
+        with cuda.stream(stream or cuda.current_stream(index)):
+            workspace = torch.torch.empty(size, dtype=torch.torch.uint8, device=groups.device)
+    _call_on(index, stream, lib().hkv_group_tokens, n, g, ids, num_groups, f, p, r,
              workspace.data_ptr(), size)
 
 
 def _positions(n, positions):
     """(address, slots) of the int32 positions [tokens, slots]."""
-    import torch
-
-    _refuse_unless(positions.dim() == 2 and positions.shape[1] > 0,
-                   "positions must be [tokens, slots]")
-    _refuse_unless(n <= positions.shape[0],
-                   f"positions has {positions.shape[0]} tokens, fewer than {n}")
-    return _list(positions, "positions", 0, torch.int32), positions.shape[1]
+    shape = positions.shape
+    _refuse_unless(len(shape) == 2 and shape[1] > 0, "positions must be [tokens, slots]")
+    if n > shape[0]:
+        raise HkvException(f"positions has {shape[0]} tokens, fewer than {n}")
+    return _list(positions, "positions", 0, _torch().int32), shape[1]
 
 
 def dispatch_rows(n, x, positions, rows, stream=None):
@@ -914,21 +927,24 @@ def dispatch_rows(n, x, positions, rows, stream=None):
     _, dim, x_stride = _matrix(x, "x", n)
     num_rows, width, rows_stride = _matrix(rows, "rows")
     _refuse_unless(width == dim and rows.dtype == x.dtype, "x and rows differ in dim or type")
-    kind = _row_types()[0].get(x.dtype)
-    _refuse_unless(kind is not None, f"rows of {x.dtype} are not supported")
+    kind = _torch().rows.get(x.dtype)
+    if kind is None:
+        raise HkvException(f"rows of {x.dtype} are not supported")
     p, slots = _positions(n, positions)
-    device = _one_device((x, positions, rows))
-    _call_on(device, stream, lib().hkv_dispatch_rows, n, slots, dim, kind, x.data_ptr(),
+    index = _one_device((x, positions, rows))
+    _call_on(index, stream, lib().hkv_dispatch_rows, n, slots, dim, kind, x.data_ptr(),
              x_stride, p, num_rows, rows.data_ptr(), rows_stride)
 
 
 def _weights(weights, name, n, slots, kind):
-    _refuse_unless(weights.dim() == 2 and weights.shape[1] == slots and weights.shape[0] >= n,
+    shape, got = weights.shape, _torch().rows.get(weights.dtype)
+    if (len(shape) == 2 and shape[1] == slots and shape[0] >= n and weights.is_contiguous()
+            and (got == 0 or got == kind)):
+        return got
+    _refuse_unless(len(shape) == 2 and shape[1] == slots and shape[0] >= n,
                    f"{name} must be [tokens, slots]")
     _refuse_unless(weights.is_contiguous(), f"{name} must be contiguous")
-    got = _row_types()[0].get(weights.dtype)
-    _refuse_unless(got in (0, kind), f"{name} must be float32 or of the rows' type")
-    return got
+    raise HkvException(f"{name} must be float32 or of the rows' type")
 
 
 def _by_place(slots, *shaped):
@@ -952,8 +968,9 @@ def combine_rows(n, rows, positions, weights, out, stream=None, slots=None):
     num_rows, dim, rows_stride = _matrix(rows, "rows")
     _, width, out_stride = _matrix(out, "out", n)
     _refuse_unless(width == dim and rows.dtype == out.dtype, "rows and out differ in dim or type")
-    kind = _row_types()[0].get(rows.dtype)
-    _refuse_unless(kind is not None, f"rows of {rows.dtype} are not supported")
+    kind = _torch().rows.get(rows.dtype)
+    if kind is None:
+        raise HkvException(f"rows of {rows.dtype} are not supported")
     tensors = [rows, out]
     if positions is not None:
         p, slots = _positions(n, positions)
@@ -965,8 +982,8 @@ def combine_rows(n, rows, positions, weights, out, stream=None, slots=None):
         w_kind = _weights(weights, "weights", n, slots, kind)
         w = weights.data_ptr()
         tensors.append(weights)
-    device = _one_device(tensors)
-    _call_on(device, stream, lib().hkv_combine_rows, n, slots, dim, kind, rows.data_ptr(),
+    index = _one_device(tensors)
+    _call_on(index, stream, lib().hkv_combine_rows, n, slots, dim, kind, rows.data_ptr(),
              rows_stride, num_rows, p, w, w_kind or 0, out.data_ptr(), out_stride)
 
 
@@ -980,8 +997,9 @@ def combine_rows_backward(n, rows, positions, weights, grad_out, grad_rows=None,
     as given or those of weights or grad_weights."""
     _refuse_unless(n >= 0, "n must not be negative")
     _, dim, out_stride = _matrix(grad_out, "grad_out", n)
-    kind = _row_types()[0].get(grad_out.dtype)
-    _refuse_unless(kind is not None, f"rows of {grad_out.dtype} are not supported")
+    kind = _torch().rows.get(grad_out.dtype)
+    if kind is None:
+        raise HkvException(f"rows of {grad_out.dtype} are not supported")
     _refuse_unless(rows is not None or grad_weights is None, "grad_weights needs rows")
     if grad_rows is None and grad_weights is None:
         return
@@ -1012,8 +1030,8 @@ def combine_rows_backward(n, rows, positions, weights, grad_out, grad_rows=None,
     if weights is not None and grad_weights is not None:
         _refuse_unless(weights.dtype == grad_weights.dtype,
                        "weights and grad_weights differ in type")
-    device = _one_device(tensors)
-    _call_on(device, stream, lib().hkv_combine_rows_backward, n, slots, dim, kind, _ptr(rows),
+    index = _one_device(tensors)
+    _call_on(index, stream, lib().hkv_combine_rows_backward, n, slots, dim, kind, _ptr(rows),
              rows_stride, num_rows, p, _ptr(weights), w_kind, grad_out.data_ptr(), out_stride,
              _ptr(grad_rows), grad_stride, _ptr(grad_weights))
 
@@ -1081,11 +1099,13 @@ class PagePool:
             lengths = torch.zeros(num_rows, dtype=torch.int32, device=device)
         self.planes, self.refs, self.table, self.lengths = planes, refs, table, lengths
         self.page_tokens, self.num_pages, self.device = page_tokens, num_pages, device
+        _torch()
+        self._index = refs.get_device()
         self._table_stride = stride
         o = _PagesOptions(num_pages=num_pages, page_tokens=page_tokens, num_rows=num_rows,
                           max_pages=max_pages, table_stride=stride, refs=refs.data_ptr(),
                           table=table.data_ptr(), lengths=lengths.data_ptr(),
-                          num_planes=len(planes), device_id=device.index)
+                          num_planes=len(planes), device_id=self._index)
         o.planes = (_P * max(len(planes), 1))(*[t.data_ptr() for t in planes])
         o.page_bytes = (_U64 * max(len(planes), 1))(
             *[t.numel() // num_pages * t.element_size() for t in planes])
@@ -1108,18 +1128,14 @@ class PagePool:
             pass
 
     def _on_stream(self, stream):
-        if stream is None:
-            import torch
+        return _TORCH.stream(self._index) if stream is None else _stream(stream)
 
-            return torch.cuda.current_stream(self.device).cuda_stream
-        return _stream(stream)
-
-    def _numbers(self, t, name, n):
-        import torch
-
-        _refuse_unless(0 <= n, "n must not be negative")
-        address = _list(t, name, n, torch.int32)
-        _refuse_unless(t.device == self.device, f"{name} is not on the pool's device")
+    def _numbers(self, t, name, n, dtype=None):
+        if n < 0:
+            raise HkvException("n must not be negative")
+        address = _list(t, name, n, dtype or _TORCH.int32)
+        if t.get_device() != self._index:
+            raise HkvException(f"{name} is not on the pool's device")
         return address
 
     def copy(self, n, src, dst, stream=None):
@@ -1140,12 +1156,7 @@ class PagePool:
         number first, copies a shared last page before the row writes behind its
         old length, or gives pages back. status (bool, optional): whether the
         entry was served; one that was not leaves its row as it was."""
-        import torch
-
-        s = None
-        if status is not None:
-            s = _list(status, "status", n, torch.bool)
-            _refuse_unless(status.device == self.device, "status is not on the pool's device")
+        s = None if status is None else self._numbers(status, "status", n, _TORCH.bool)
         _check(lib().hkv_pages_resize(self._h, n, self._numbers(rows, "rows", n),
                                       self._numbers(lengths, "lengths", n), s,
                                       self._on_stream(stream)))
