@@ -10,12 +10,11 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
-#include "hkv_table.cuh"
+#include "hkv_ops.cuh"
 
 namespace hkvb {
-
-void set_last_error(const std::string& m);
 
 namespace {
 
@@ -87,6 +86,7 @@ template <int kBytes>
 __global__ void __launch_bounds__(kCopyThreads)
     copy_pages_kernel(const __grid_constant__ PlaneSet planes, uint32_t num_pages,
                       const int32_t* src, const int32_t* dst) {
+  after_previous();
   const uint32_t pair = blockIdx.x / planes.chunks, c = blockIdx.x - pair * planes.chunks;
   const uint32_t s = static_cast<uint32_t>(src[pair]), d = static_cast<uint32_t>(dst[pair]);
   if (s >= num_pages || d >= num_pages || s == d) return;
@@ -118,6 +118,7 @@ struct Fork {
 __global__ void __launch_bounds__(kForkThreads)
     fork_read_kernel(PoolView v, uint32_t n, const int32_t* src, const int32_t* dst, Fork* forks,
                      int32_t* staged) {
+  after_previous();
   const uint32_t e = blockIdx.x;
   const int32_t s = src[e], d = dst[e];
   bool on = static_cast<uint32_t>(s) < v.num_rows && static_cast<uint32_t>(d) < v.num_rows;
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(kForkThreads)
 
 __global__ void __launch_bounds__(kForkThreads)
     fork_write_kernel(PoolView v, const int32_t* dst, const Fork* forks, const int32_t* staged) {
+  after_previous();
   const uint32_t e = blockIdx.x;
   const Fork f = forks[e];
   if (f.length < 0) return;
@@ -155,6 +157,7 @@ __global__ void __launch_bounds__(kForkThreads)
 // ---- free and hold ----------------------------------------------------------
 
 __global__ void __launch_bounds__(256) free_rows_kernel(PoolView v, const int32_t* rows) {
+  after_previous();
   const uint32_t r = static_cast<uint32_t>(rows[blockIdx.x]);
   if (r >= v.num_rows) return;
   __shared__ int32_t length;
@@ -169,6 +172,7 @@ __global__ void __launch_bounds__(256) free_rows_kernel(PoolView v, const int32_
 
 __global__ void __launch_bounds__(256)
     hold_kernel(PoolView v, uint64_t n, const int32_t* pages, int delta) {
+  after_previous();
   const uint64_t i = blockIdx.x * static_cast<uint64_t>(blockDim.x) + threadIdx.x;
   if (i >= n) return;
   const uint32_t page = static_cast<uint32_t>(pages[i]);
@@ -195,34 +199,6 @@ __device__ __forceinline__ uint32_t free_bits(int4 c) {
 }
 __device__ __forceinline__ uint32_t live_bits(int4 c) {
   return (c.x > 0) | (c.y > 0) << 1 | (c.z > 0) << 2 | (c.w > 0) << 3;
-}
-
-// Exclusive sum of u over the block's threads, and the sum of all.
-__device__ __forceinline__ uint32_t block_exclusive(uint32_t u, uint32_t* total) {
-  __shared__ uint32_t sums[33];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t inc = u;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t w = __shfl_up_sync(~0u, inc, o);
-    if (lane >= o) inc += w;
-  }
-  __syncthreads();
-  if (lane == 31) sums[warp] = inc;
-  __syncthreads();
-  if (warp == 0) {
-    const int warps = blockDim.x >> 5;
-    uint32_t w = lane < warps ? sums[lane] : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t x = __shfl_up_sync(~0u, w, o);
-      if (lane >= o) w += x;
-    }
-    sums[lane] = w;
-  }
-  __syncthreads();
-  *total = sums[(blockDim.x >> 5) - 1];
-  return (warp ? sums[warp - 1] : 0) + inc - u;
 }
 
 // sums of counts[0 .. strip) and of counts[0 .. strips)
@@ -255,6 +231,7 @@ constexpr uint32_t kStripWarps = kStripThreads / 32;
 __global__ void __launch_bounds__(kStripThreads)
     resize_count_kernel(PoolView v, uint32_t n, const int32_t* rows, const int32_t* lengths,
                         uint32_t strips, uint32_t* counts, Want* wants, uint32_t* needs) {
+  after_previous();
   if (blockIdx.x < strips) {
     uint32_t first, total;
     const int4 c = strip_counts(v, blockIdx.x, &first);
@@ -290,6 +267,7 @@ __global__ void __launch_bounds__(kStripThreads)
 __global__ void __launch_bounds__(kStripThreads)
     resize_list_kernel(PoolView v, uint32_t n, uint32_t strips, const uint32_t* counts,
                        const uint32_t* needs, uint32_t* first_of, int32_t* free_list) {
+  after_previous();
   if (blockIdx.x == strips) {  // places in the list, in the entries' order
     uint32_t free, ignored, run = 0;
     strip_base(counts, strips, strips, &free, &ignored);
@@ -323,6 +301,7 @@ template <int kBytes>
 __global__ void __launch_bounds__(kCopyThreads)
     resize_apply_kernel(const __grid_constant__ PlaneSet planes, PoolView v, const Want* wants,
                         const uint32_t* first_of, const int32_t* free_list, bool* status) {
+  after_previous();
   const uint32_t e = blockIdx.x;
   const Want w = wants[e];
   const uint32_t first = first_of[e];
@@ -367,6 +346,7 @@ __global__ void __launch_bounds__(kCopyThreads)
 
 __global__ void __launch_bounds__(kStripThreads)
     compact_count_kernel(PoolView v, uint32_t* counts) {
+  after_previous();
   uint32_t first, total;
   const int4 c = strip_counts(v, blockIdx.x, &first);
   block_exclusive(__popc(live_bits(c)), &total);
@@ -381,6 +361,7 @@ struct Compact {
 __global__ void __launch_bounds__(kStripThreads)
     compact_list_kernel(PoolView v, uint32_t strips, const uint32_t* counts, int32_t* page_map,
                         int32_t* holes, int32_t* movers, int32_t* refs_out, Compact* result) {
+  after_previous();
   uint32_t before, live, ignored, first;
   strip_base(counts, blockIdx.x, strips, &before, &live);
   const int4 c = strip_counts(v, blockIdx.x, &first);
@@ -422,6 +403,7 @@ __global__ void __launch_bounds__(kCopyThreads)
     compact_move_kernel(const __grid_constant__ PlaneSet planes, PoolView v, int32_t* page_map,
                         const int32_t* holes, const int32_t* movers, const int32_t* refs,
                         int32_t* refs_out, int32_t* table_out, const Compact* result) {
+  after_previous();
   const uint32_t live = result->live, below = result->below, moved = live - below;
   const uint32_t row_chunks = (v.max_pages + kTableChunk - 1) / kTableChunk;
   const uint64_t table_units = static_cast<uint64_t>(v.num_rows) * row_chunks;
@@ -573,15 +555,10 @@ class PagesImpl {
     const size_t most = 0x7fffffff / planes_.chunks;  // pairs of a launch
     for (size_t i = 0; i < n; i += most) {
       const uint32_t blocks = static_cast<uint32_t>(std::min(most, n - i)) * planes_.chunks;
-      const int32_t *a = src + i, *b = dst + i;
-      const uint32_t pages = view_.num_pages;
-      if (width_ == 16)
-        copy_pages_kernel<16><<<blocks, kCopyThreads, 0, counted(s)>>>(planes_, pages, a, b);
-      else if (width_ == 4)
-        copy_pages_kernel<4><<<blocks, kCopyThreads, 0, counted(s)>>>(planes_, pages, a, b);
-      else
-        copy_pages_kernel<1><<<blocks, kCopyThreads, 0, counted(s)>>>(planes_, pages, a, b);
-      CUDA_TRY(cudaGetLastError());
+      with_width([&](auto width) {
+        launch(copy_pages_kernel<decltype(width)::value>, blocks, kCopyThreads, 0, s, 1, planes_,
+               view_.num_pages, src + i, dst + i);
+      });
     }
   }
 
@@ -592,11 +569,9 @@ class PagesImpl {
     check_list(dst, "dst");
     OnDevice on(device_);
     const dim3 grid(static_cast<uint32_t>(n), (view_.max_pages + kForkChunk - 1) / kForkChunk);
-    fork_read_kernel<<<grid, kForkThreads, 0, counted(s)>>>(view_, static_cast<uint32_t>(n), src,
-                                                            dst, forks_, staged_);
-    CUDA_TRY(cudaGetLastError());
-    fork_write_kernel<<<grid, kForkThreads, 0, counted(s)>>>(view_, dst, forks_, staged_);
-    CUDA_TRY(cudaGetLastError());
+    launch(fork_read_kernel, grid, kForkThreads, 0, s, 1, view_, static_cast<uint32_t>(n), src, dst,
+           forks_, staged_);
+    launch(fork_write_kernel, grid, kForkThreads, 0, s, 1, view_, dst, forks_, staged_);
   }
 
   void resize(size_t n, const int32_t* rows, const int32_t* lengths, bool* status,
@@ -607,27 +582,18 @@ class PagesImpl {
     check_list(lengths, "lengths");
     OnDevice on(device_);
     const uint32_t m = static_cast<uint32_t>(n);
-    resize_count_kernel<<<strips_ + (m + kStripWarps - 1) / kStripWarps, kStripThreads, 0,
-                          counted(s)>>>(view_, m, rows, lengths, strips_, counts_, wants_,
-                                        needs_);
-    CUDA_TRY(cudaGetLastError());
-    resize_list_kernel<<<strips_ + 1, kStripThreads, 0, counted(s)>>>(view_, m, strips_, counts_,
-                                                                      needs_, first_, list_);
-    CUDA_TRY(cudaGetLastError());
+    launch(resize_count_kernel, strips_ + (m + kStripWarps - 1) / kStripWarps, kStripThreads, 0, s,
+           1, view_, m, rows, lengths, strips_, counts_, wants_, needs_);
+    launch(resize_list_kernel, strips_ + 1, kStripThreads, 0, s, 1, view_, m, strips_, counts_,
+           needs_, first_, list_);
     // blocks of an entry: as many as its page copy can use, few where there
     // are entries enough to fill the device
     const uint32_t fill = std::max(1u, static_cast<uint32_t>(sm_count_) * 16 / m);
     const dim3 grid(m, std::max(1u, std::min(planes_.chunks, fill)));
-    if (width_ == 16)
-      resize_apply_kernel<16><<<grid, kCopyThreads, 0, counted(s)>>>(planes_, view_, wants_,
-                                                                     first_, list_, status);
-    else if (width_ == 4)
-      resize_apply_kernel<4><<<grid, kCopyThreads, 0, counted(s)>>>(planes_, view_, wants_,
-                                                                    first_, list_, status);
-    else
-      resize_apply_kernel<1><<<grid, kCopyThreads, 0, counted(s)>>>(planes_, view_, wants_,
-                                                                    first_, list_, status);
-    CUDA_TRY(cudaGetLastError());
+    with_width([&](auto width) {
+      launch(resize_apply_kernel<decltype(width)::value>, grid, kCopyThreads, 0, s, 1, planes_,
+             view_, wants_, first_, list_, status);
+    });
   }
 
   void free_rows(size_t n, const int32_t* rows, cudaStream_t s) {
@@ -635,8 +601,7 @@ class PagesImpl {
     if (n == 0) return;
     check_list(rows, "rows");
     OnDevice on(device_);
-    free_rows_kernel<<<static_cast<uint32_t>(n), 256, 0, counted(s)>>>(view_, rows);
-    CUDA_TRY(cudaGetLastError());
+    launch(free_rows_kernel, static_cast<uint32_t>(n), 256, 0, s, 1, view_, rows);
   }
 
   void hold(size_t n, const int32_t* pages, int delta, cudaStream_t s) {
@@ -644,9 +609,8 @@ class PagesImpl {
     if (n == 0) return;
     check_list(pages, "pages");
     OnDevice on(device_);
-    hold_kernel<<<static_cast<uint32_t>((n + 255) / 256), 256, 0, counted(s)>>>(view_, n, pages,
-                                                                                delta);
-    CUDA_TRY(cudaGetLastError());
+    launch(hold_kernel, static_cast<uint32_t>((n + 255) / 256), 256, 0, s, 1, view_, n, pages,
+           delta);
   }
 
   void compact(int32_t* page_map, int32_t* table_out, int32_t* refs_out, cudaStream_t s) {
@@ -654,27 +618,19 @@ class PagesImpl {
     if (table_out) check_list(table_out, "table_out"); else table_out = view_.table;
     if (refs_out) check_list(refs_out, "refs_out"); else refs_out = view_.refs;
     OnDevice on(device_);
-    compact_count_kernel<<<strips_, kStripThreads, 0, counted(s)>>>(view_, counts_);
-    CUDA_TRY(cudaGetLastError());
-    compact_list_kernel<<<strips_, kStripThreads, 0, counted(s)>>>(
-        view_, strips_, counts_, page_map, list_, movers_, refs_out, result_);
-    CUDA_TRY(cudaGetLastError());
+    launch(compact_count_kernel, strips_, kStripThreads, 0, s, 1, view_, counts_);
+    launch(compact_list_kernel, strips_, kStripThreads, 0, s, 1, view_, strips_, counts_, page_map,
+           list_, movers_, refs_out, result_);
     // at most half of the pages can move
     const uint64_t units = (view_.num_pages / 2 + 1ull) * (planes_.chunks + 1ull) +
                            static_cast<uint64_t>(view_.num_rows) *
                                ((view_.max_pages + kTableChunk - 1) / kTableChunk);
     const uint32_t grid =
         static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(sm_count_) * 8, units));
-    if (width_ == 16)
-      compact_move_kernel<16><<<grid, kCopyThreads, 0, counted(s)>>>(
-          planes_, view_, page_map, list_, movers_, view_.refs, refs_out, table_out, result_);
-    else if (width_ == 4)
-      compact_move_kernel<4><<<grid, kCopyThreads, 0, counted(s)>>>(
-          planes_, view_, page_map, list_, movers_, view_.refs, refs_out, table_out, result_);
-    else
-      compact_move_kernel<1><<<grid, kCopyThreads, 0, counted(s)>>>(
-          planes_, view_, page_map, list_, movers_, view_.refs, refs_out, table_out, result_);
-    CUDA_TRY(cudaGetLastError());
+    with_width([&](auto width) {
+      launch(compact_move_kernel<decltype(width)::value>, grid, kCopyThreads, 0, s, 1, planes_,
+             view_, page_map, list_, movers_, view_.refs, refs_out, table_out, result_);
+    });
   }
 
  private:
@@ -682,11 +638,17 @@ class PagesImpl {
   void check_count(size_t n) const {
     HKV_REQUIRE(n <= view_.num_rows, HKV_ERR_INVALID, "more entries than the pool has rows");
   }
-  static void check_list(const int32_t* p, const char* what) {
-    HKV_REQUIRE(p != nullptr, HKV_ERR_INVALID, std::string(what) + " is null");
-    HKV_REQUIRE(reinterpret_cast<uintptr_t>(p) % 4 == 0, HKV_ERR_INVALID,
-                std::string(what) + " is not aligned to its elements");
+  // calls f with the pool's word width as a constant
+  template <class F>
+  void with_width(F f) const {
+    if (width_ == 16)
+      f(std::integral_constant<int, 16>{});
+    else if (width_ == 4)
+      f(std::integral_constant<int, 4>{});
+    else
+      f(std::integral_constant<int, 1>{});
   }
+  static void check_list(const int32_t* p, const char* what) { require(p, 4, what); }
 
   MemSource mem_;
   PlaneSet planes_{};
@@ -713,21 +675,6 @@ struct hkv_pages {
 // ===========================================================================
 // C ABI
 // ===========================================================================
-using hkvb::HkvError;
-
-#define HKV_API_BEGIN try {
-#define HKV_API_END                     \
-  return HKV_OK;                        \
-  }                                     \
-  catch (const HkvError& e) {           \
-    hkvb::set_last_error(e.msg);        \
-    return e.code;                      \
-  }                                     \
-  catch (const std::exception& e) {     \
-    hkvb::set_last_error(e.what());     \
-    return HKV_ERR_RUNTIME;             \
-  }
-
 #define HKV_PAGES(p)                                                    \
   HKV_REQUIRE((p) != nullptr && (p)->impl != nullptr, HKV_ERR_INVALID,  \
               "null pool");                                             \

@@ -12,11 +12,9 @@
 #include <string>
 #include <type_traits>
 
-#include "hkv_table.cuh"
+#include "hkv_ops.cuh"
 
 namespace hkvb {
-
-void set_last_error(const std::string& m);
 
 namespace {
 
@@ -38,12 +36,15 @@ struct FastDiv {
 };
 
 // ---- sort by group ----------------------------------------------------------
-
-constexpr int kSortThreads = 512;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortItems = 8;  // places of a thread and tile
-constexpr int kSortTile = kSortThreads * kSortItems;
-constexpr uint32_t kSortBlocks = 592;  // 4 x 148: blocks of the long form
+// A counting sort that keeps the order of equal ids. A warp takes a run of
+// 32 * kItems places; __match_any_sync ranks each place among the equal ids of
+// its warp step, the warp's own count of the id among the steps before. The
+// warps' counts, scanned over the warps, and the start of the group in this
+// block's part make the row.
+//
+// Two forms, chosen by n and num_groups (see sort_plan): one launch of one
+// cluster, whose blocks exchange their counts through distributed shared
+// memory; and three launches with the counts in global memory.
 
 template <class Id>
 __device__ __forceinline__ int load_group(const void* groups, uint64_t i, uint64_t n,
@@ -53,44 +54,162 @@ __device__ __forceinline__ int load_group(const void* groups, uint64_t i, uint64
   return id >= 0 && id < static_cast<Id>(num_groups) ? static_cast<int>(id) : -1;
 }
 
-// Exclusive sum of v over the block's threads, and the sum of all.
-__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* warp_sums,
-                                                    uint32_t* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  uint32_t inc = v;
+// Ranks of a warp's places; mine[g] counts the warp's places of group g.
+template <int kItems>
+__device__ __forceinline__ void rank_in_warp(const int (&id)[kItems], uint16_t* mine,
+                                             uint32_t (&rank)[kItems]) {
+  const uint32_t below = (1u << (threadIdx.x & 31)) - 1;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t u = __shfl_up_sync(~0u, inc, o);
-    if (lane >= o) inc += u;
+  for (int it = 0; it < kItems; it++) {
+    const uint32_t same = __match_any_sync(~0u, id[it]);
+    const uint32_t before = id[it] >= 0 ? mine[id[it]] : 0;
+    rank[it] = before + __popc(same & below);
+    __syncwarp();
+    if (id[it] >= 0 && (same & below) == 0) mine[id[it]] = before + __popc(same);
+    __syncwarp();
   }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = inc;
-  __syncthreads();
-  uint32_t before = 0, all = 0;
-  for (int w = 0; w < warps; w++) {
-    const uint32_t u = warp_sums[w];
-    if (w < warp) before += u;
-    all += u;
-  }
-  *total = all;
-  return before + inc - v;
 }
 
-// counts[g * blocks + b]: the places of group g in block b's run of tiles
-template <class Id>
+// cnt[w][g] becomes the places of group g in the warps before w; returns all.
+__device__ __forceinline__ uint32_t scan_over_warps(uint16_t* cnt, uint32_t warps,
+                                                    uint32_t num_groups, uint32_t g) {
+  uint32_t before = 0;
+#pragma unroll 8
+  for (uint32_t w = 0; w < warps; w++) {
+    const uint32_t c = cnt[w * num_groups + g];
+    cnt[w * num_groups + g] = before;
+    before += c;
+  }
+  return before;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n"
+               "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// word `p` of this block's shared memory, in block `rank` of the cluster
+__device__ __forceinline__ uint32_t load_remote(const uint32_t* p, uint32_t rank) {
+  uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(p)), r, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(r) : "memory");
+  return v;
+}
+
+// One launch: `blocks` blocks of one cluster, block b takes the places from
+// b * blockDim.x * kItems. The rows of order are written from shared memory
+// in the block's sorted order, so that a group's run is written in whole
+// sectors.
+constexpr uint32_t kClusterThreads = 1024;
+
+template <class Id, int kItems>
+__global__ void __launch_bounds__(kClusterThreads)
+    group_cluster_kernel(uint32_t n, const void* groups, uint32_t num_groups, uint32_t blocks,
+                         int32_t* offsets, int32_t* positions, int32_t* order) {
+  extern __shared__ uint32_t smem[];
+  const uint32_t threads = blockDim.x, warps = threads / 32, me = blocks > 1 ? cluster_rank() : 0;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t* mine_all = smem;               // [num_groups] places of a group in this block
+  uint32_t* start = mine_all + num_groups;  // [num_groups] first row in this block
+  uint32_t* local = start + num_groups;     // [num_groups] the same in the block's own order
+  uint2* staged = reinterpret_cast<uint2*>(local + num_groups + (num_groups & 1));
+  uint16_t* cnt = reinterpret_cast<uint16_t*>(staged + (order ? threads * kItems : 0));
+  for (uint32_t k = threadIdx.x; k < num_groups * warps / 2; k += threads)
+    reinterpret_cast<uint32_t*>(cnt)[k] = 0;  // warps is even
+  after_previous();
+  const uint32_t base = (me * warps + warp) * 32 * kItems + lane;
+  int id[kItems];
+  uint32_t rank[kItems];
+#pragma unroll
+  for (int it = 0; it < kItems; it++) id[it] = load_group<Id>(groups, base + it * 32, n, num_groups);
+  __syncthreads();
+  uint16_t* mine = cnt + warp * num_groups;
+  rank_in_warp(id, mine, rank);
+  __syncthreads();
+  for (uint32_t g = threadIdx.x; g < num_groups; g += threads)
+    mine_all[g] = scan_over_warps(cnt, warps, num_groups, g);
+  if (blocks > 1) cluster_sync();
+  __syncthreads();
+  // starts, over contiguous runs of groups per thread
+  const uint32_t per = (num_groups + threads - 1) / threads;
+  const uint32_t g0 = min(num_groups, threadIdx.x * per), g1 = min(num_groups, g0 + per);
+  uint32_t sum = 0, own = 0, kept, here;
+  for (uint32_t g = g0; g < g1; g++) {
+    uint32_t before = 0, all = 0;
+#pragma unroll 4
+    for (uint32_t b = 0; b < blocks; b++) {
+      const uint32_t c = blocks > 1 ? load_remote(mine_all + g, b) : mine_all[g];
+      if (b < me) before += c;
+      all += c;
+    }
+    start[g] = before;
+    local[g] = all;  // for now
+    sum += all;
+    own += mine_all[g];
+  }
+  uint32_t run = block_exclusive(sum, &kept);
+  uint32_t run_here = block_exclusive(own, &here);
+  for (uint32_t g = g0; g < g1; g++) {
+    if (me == 0) offsets[g] = run;
+    start[g] += run;
+    run += local[g];
+    local[g] = run_here;
+    run_here += mine_all[g];
+  }
+  if (me == 0 && threadIdx.x == 0) offsets[num_groups] = kept;
+  __syncthreads();
+#pragma unroll
+  for (int it = 0; it < kItems; it++) {
+    const uint32_t i = base + it * 32;
+    if (i >= n) continue;
+    uint32_t row = ~0u;
+    if (id[it] >= 0) {
+      const uint32_t at = mine[id[it]] + rank[it];
+      row = start[id[it]] + at;
+      if (order) staged[local[id[it]] + at] = make_uint2(row, i);
+    }
+    positions[i] = row;
+  }
+  if (order) {
+    __syncthreads();
+    for (uint32_t k = threadIdx.x; k < here; k += threads) order[staged[k].x] = staged[k].y;
+    for (uint32_t k = kept + me * threads + threadIdx.x; k < n; k += blocks * threads) order[k] = -1;
+  }
+  if (blocks > 1) cluster_sync();  // until all have read this block's counts
+}
+
+// Three launches. Blocks take runs of tiles; counts[g * blocks + b].
+
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr uint32_t kSortBlocks = 592;  // 4 x 148
+
+template <class Id, int kItems>
 __global__ void __launch_bounds__(kSortThreads)
     group_count_kernel(uint64_t n, const void* groups, uint32_t num_groups,
                        uint32_t tiles_per_block, uint32_t* counts) {
   extern __shared__ uint32_t hist[];
   for (uint32_t g = threadIdx.x; g < num_groups; g += blockDim.x) hist[g] = 0;
   __syncthreads();
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * tiles_per_block * kSortTile;
-  const uint64_t last = min(n, first + static_cast<uint64_t>(tiles_per_block) * kSortTile);
+  after_previous();
+  constexpr uint64_t kTile = kSortThreads * kItems;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * tiles_per_block * kTile;
+  const uint64_t last = min(n, first + tiles_per_block * kTile);
   const uint32_t below = (1u << (threadIdx.x & 31)) - 1;
-  for (uint64_t base = first; base < last; base += kSortThreads) {
-    const int id = load_group<Id>(groups, base + threadIdx.x, last, num_groups);
-    const uint32_t same = __match_any_sync(~0u, id);
-    if (id >= 0 && (same & below) == 0) atomicAdd(&hist[id], __popc(same));
+  for (uint64_t base = first; base < last; base += kTile) {
+    int id[kItems];
+#pragma unroll
+    for (int it = 0; it < kItems; it++)
+      id[it] = load_group<Id>(groups, base + it * kSortThreads + threadIdx.x, last, num_groups);
+#pragma unroll
+    for (int it = 0; it < kItems; it++) {
+      const uint32_t same = __match_any_sync(~0u, id[it]);
+      if (id[it] >= 0 && (same & below) == 0) atomicAdd(&hist[id[it]], __popc(same));
+    }
   }
   __syncthreads();
   for (uint32_t g = threadIdx.x; g < num_groups; g += blockDim.x)
@@ -100,6 +219,7 @@ __global__ void __launch_bounds__(kSortThreads)
 // a warp per group: its counts become the places in earlier blocks, and the sum
 __global__ void group_scan_kernel(uint32_t num_groups, uint32_t blocks, uint32_t* counts,
                                   uint32_t* totals) {
+  after_previous();
   const uint32_t g = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (g >= num_groups) return;
@@ -119,30 +239,26 @@ __global__ void group_scan_kernel(uint32_t num_groups, uint32_t blocks, uint32_t
   if (lane == 0) totals[g] = run;
 }
 
-// Ranks the places of a block's tiles. A warp takes a run of 32 * kSortItems
-// places; __match_any_sync gives each place its rank among the equal ids of its
-// warp step, the warp's count of the id what came before. The counts of the
-// block's warps, scanned over the warps, and the start of the group make the
-// row.
-template <class Id>
+template <class Id, int kItems>
 __global__ void __launch_bounds__(kSortThreads)
     group_place_kernel(uint64_t n, const void* groups, uint32_t num_groups,
                        uint32_t tiles_per_block, const uint32_t* counts,
                        const uint32_t* totals, int32_t* offsets, int32_t* positions,
                        int32_t* order) {
   extern __shared__ uint32_t smem[];
-  __shared__ uint32_t warp_sums[32];
   uint32_t* start = smem;  // [num_groups]
   uint16_t* cnt = reinterpret_cast<uint16_t*>(smem + num_groups);  // [kSortWarps + 1][num_groups]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t below = (1u << lane) - 1;
+  constexpr uint64_t kTile = kSortThreads * kItems;
+  after_previous();
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * tiles_per_block;
 
   // start of each group, over contiguous runs of groups per thread
   const uint32_t per = (num_groups + kSortThreads - 1) / kSortThreads;
   const uint32_t g0 = min(num_groups, threadIdx.x * per), g1 = min(num_groups, g0 + per);
   uint32_t sum = 0, kept = 0;
   for (uint32_t g = g0; g < g1; g++) sum += totals[g];
-  uint32_t run = block_exclusive(sum, warp_sums, &kept);
+  uint32_t run = block_exclusive(sum, &kept);
   for (uint32_t g = g0; g < g1; g++) {
     if (blockIdx.x == 0) offsets[g] = run;
     start[g] = run + counts[static_cast<uint64_t>(g) * gridDim.x + blockIdx.x];
@@ -155,41 +271,25 @@ __global__ void __launch_bounds__(kSortThreads)
          i += static_cast<uint64_t>(gridDim.x) * kSortThreads)
       order[i] = -1;
 
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * tiles_per_block;
   for (uint32_t t = 0; t < tiles_per_block; t++) {
-    const uint64_t base = (first + t) * kSortTile + warp * 32 * kSortItems;
-    if ((first + t) * kSortTile >= n) break;
+    const uint64_t base = (first + t) * kTile + warp * 32 * kItems + lane;
+    if ((first + t) * kTile >= n) break;
+    int id[kItems];
+    uint32_t rank[kItems];
+#pragma unroll
+    for (int it = 0; it < kItems; it++)
+      id[it] = load_group<Id>(groups, base + it * 32, n, num_groups);
     for (uint32_t k = threadIdx.x; k < num_groups * kSortWarps; k += kSortThreads) cnt[k] = 0;
     __syncthreads();
-    int id[kSortItems];
-    uint32_t rank[kSortItems];
-#pragma unroll
-    for (int it = 0; it < kSortItems; it++)
-      id[it] = load_group<Id>(groups, base + it * 32 + lane, n, num_groups);
     uint16_t* mine = cnt + warp * num_groups;
-#pragma unroll
-    for (int it = 0; it < kSortItems; it++) {
-      const uint32_t same = __match_any_sync(~0u, id[it]);
-      const uint32_t before = id[it] >= 0 ? mine[id[it]] : 0;
-      rank[it] = before + __popc(same & below);
-      __syncwarp();
-      if (id[it] >= 0 && (same & below) == 0) mine[id[it]] = before + __popc(same);
-      __syncwarp();
-    }
+    rank_in_warp(id, mine, rank);
     __syncthreads();
-    for (uint32_t g = threadIdx.x; g < num_groups; g += kSortThreads) {
-      uint32_t before = 0;
-      for (int w = 0; w < kSortWarps; w++) {
-        const uint32_t c = cnt[w * num_groups + g];
-        cnt[w * num_groups + g] = before;
-        before += c;
-      }
-      cnt[kSortWarps * num_groups + g] = before;
-    }
+    for (uint32_t g = threadIdx.x; g < num_groups; g += kSortThreads)
+      cnt[kSortWarps * num_groups + g] = scan_over_warps(cnt, kSortWarps, num_groups, g);
     __syncthreads();
 #pragma unroll
-    for (int it = 0; it < kSortItems; it++) {
-      const uint64_t i = base + it * 32 + lane;
+    for (int it = 0; it < kItems; it++) {
+      const uint64_t i = base + it * 32;
       if (i >= n) continue;
       if (id[it] < 0) {
         positions[i] = -1;
@@ -205,40 +305,98 @@ __global__ void __launch_bounds__(kSortThreads)
   }
 }
 
-uint32_t sort_tiles_per_block(size_t n) {
-  const size_t tiles = (n + kSortTile - 1) / kSortTile;
-  return static_cast<uint32_t>(std::max<size_t>(1, (tiles + kSortBlocks - 1) / kSortBlocks));
+struct SortPlan {
+  bool cluster;
+  uint32_t items, blocks, threads;  // of the one-launch form
+  uint32_t run;                     // tiles of a block of the long form
+  size_t smem, workspace;
+};
+
+size_t cluster_smem(uint32_t num_groups, uint32_t threads, uint32_t items) {
+  return (3ull * num_groups + (num_groups & 1)) * 4 + threads * items * 8ull +
+         static_cast<size_t>(num_groups) * (threads / 32) * 2;
 }
 
-uint32_t sort_blocks(size_t n) {
-  const size_t run = static_cast<size_t>(sort_tiles_per_block(n)) * kSortTile;
-  return static_cast<uint32_t>(std::max<size_t>(1, (n + run - 1) / run));
+constexpr uint32_t kMaxCluster = 8;
+
+SortPlan sort_plan(size_t n, uint32_t num_groups) {
+  SortPlan p{};
+  // one launch while a block's share fits its registers and shared memory
+  if (n <= static_cast<size_t>(kMaxCluster) * kClusterThreads * 16) {
+    const uint32_t m = std::max<uint32_t>(1, static_cast<uint32_t>(n));
+    p.blocks = 1;
+    while (p.blocks < kMaxCluster && m > p.blocks * kClusterThreads * 2) p.blocks *= 2;
+    p.items = 1;
+    while (p.blocks * p.items * kClusterThreads < m) p.items *= 2;
+    p.threads = kClusterThreads;
+    if (p.blocks == 1)
+      p.threads = std::max(128u, std::min(kClusterThreads, ((m + p.items - 1) / p.items + 63) / 64 * 64));
+    p.smem = cluster_smem(num_groups, p.threads, p.items);
+    p.cluster = p.smem <= 220 * 1024;
+  }
+  if (p.cluster) {
+    p.workspace = 16;
+    return p;
+  }
+  p.items = 1;
+  while (p.items < 8 && n > static_cast<size_t>(p.items) * kSortThreads * kSortBlocks / 2) p.items *= 2;
+  const size_t tile = static_cast<size_t>(kSortThreads) * p.items;
+  const size_t tiles = (n + tile - 1) / tile;
+  p.run = static_cast<uint32_t>(std::max<size_t>(1, (tiles + kSortBlocks - 1) / kSortBlocks));
+  p.blocks = static_cast<uint32_t>(std::max<size_t>(1, (tiles + p.run - 1) / p.run));
+  p.threads = kSortThreads;
+  p.smem = static_cast<size_t>(num_groups) * (4 + 2 * (kSortWarps + 1));
+  p.workspace = (static_cast<size_t>(num_groups) * p.blocks + num_groups) * 4;
+  return p;
 }
 
-size_t sort_workspace(size_t n, uint32_t num_groups) {
-  return (static_cast<size_t>(num_groups) * sort_blocks(n) + num_groups) * 4;
+// calls f with kItems as a constant
+template <class F>
+void with_items(uint32_t items, F f) {
+  switch (items) {
+    case 1: f(std::integral_constant<int, 1>{}); break;
+    case 2: f(std::integral_constant<int, 2>{}); break;
+    case 4: f(std::integral_constant<int, 4>{}); break;
+    case 8: f(std::integral_constant<int, 8>{}); break;
+    default: f(std::integral_constant<int, 16>{});
+  }
+}
+
+template <class K>
+void allow_smem(K kernel, size_t smem) {
+  if (smem > 48 * 1024)
+    CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>(smem)));
 }
 
 template <class Id>
 void launch_sort(size_t n, const void* groups, uint32_t num_groups, int32_t* offsets,
                  int32_t* positions, int32_t* order, void* workspace, cudaStream_t s) {
-  const uint32_t blocks = sort_blocks(n), run = sort_tiles_per_block(n);
-  uint32_t* counts = static_cast<uint32_t*>(workspace);
-  uint32_t* totals = counts + static_cast<size_t>(num_groups) * blocks;
-  group_count_kernel<Id><<<blocks, kSortThreads, num_groups * 4, counted(s)>>>(
-      n, groups, num_groups, run, counts);
-  CUDA_TRY(cudaGetLastError());
-  group_scan_kernel<<<(num_groups + 7) / 8, 256, 0, counted(s)>>>(num_groups, blocks, counts,
-                                                                  totals);
-  CUDA_TRY(cudaGetLastError());
-  const size_t smem = num_groups * (4 + 2 * (kSortWarps + 1));
-  if (smem > 48 * 1024)
-    CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<Id>,
-                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(smem)));
-  group_place_kernel<Id><<<blocks, kSortThreads, smem, counted(s)>>>(
-      n, groups, num_groups, run, counts, totals, offsets, positions, order);
-  CUDA_TRY(cudaGetLastError());
+  const SortPlan p = sort_plan(n, num_groups);
+  with_items(p.items, [&](auto items) {
+    constexpr int kItems = decltype(items)::value;
+    if (p.cluster) {
+      auto kernel = group_cluster_kernel<Id, kItems>;
+      allow_smem(kernel, p.smem);
+      launch(kernel, p.blocks, p.threads, p.smem, s, p.blocks, static_cast<uint32_t>(n), groups,
+             num_groups, p.blocks, offsets, positions, order);
+      return;
+    }
+    if constexpr (kItems <= 8) {
+      uint32_t* counts = static_cast<uint32_t*>(workspace);
+      uint32_t* totals = counts + static_cast<size_t>(num_groups) * p.blocks;
+      const uint64_t n64 = n;
+      launch(group_count_kernel<Id, kItems>, p.blocks, kSortThreads, num_groups * 4, s, 1, n64,
+             groups, num_groups, p.run, counts);
+      launch(group_scan_kernel, (num_groups + 7) / 8, 256, 0, s, 1, num_groups, p.blocks, counts,
+             totals);
+      auto kernel = group_place_kernel<Id, kItems>;
+      allow_smem(kernel, p.smem);
+      launch(kernel, p.blocks, kSortThreads, p.smem, s, 1, n64, groups, num_groups, p.run,
+             static_cast<const uint32_t*>(counts), static_cast<const uint32_t*>(totals), offsets,
+             positions, order);
+    }
+  });
 }
 
 // ---- rows -------------------------------------------------------------------
@@ -261,6 +419,7 @@ __global__ void __launch_bounds__(kRowThreads)
                     uint64_t x_stride, const int32_t* positions, uint32_t num_rows, void* rows,
                     uint64_t rows_stride) {
   using T = typename Word<kBytes>::type;
+  after_previous();
   const uint32_t i = blockIdx.x * kRowThreads + threadIdx.x;
   if (i >= words_of_all) return;
   const uint32_t t = words.div(i), c = i - t * words.d;
@@ -297,6 +456,7 @@ __global__ void __launch_bounds__(kRowThreads)
     combine_kernel(uint32_t packs_of_all, FastDiv packs, uint32_t slots, const T* rows,
                    uint64_t rows_stride, uint32_t num_rows, const int32_t* positions,
                    const W* weights, T* out, uint64_t out_stride) {
+  after_previous();
   const uint32_t i = blockIdx.x * kRowThreads + threadIdx.x;
   if (i >= packs_of_all) return;
   const uint32_t t = packs.div(i), c = (i - t * packs.d) * kVec;
@@ -327,6 +487,7 @@ __global__ void __launch_bounds__(kRowThreads)
                             uint64_t rows_stride, uint32_t num_rows, const int32_t* positions,
                             const W* weights, const T* grad_out, uint64_t grad_out_stride,
                             T* grad_rows, uint64_t grad_rows_stride, W* grad_weights) {
+  after_previous();
   const uint32_t i = (blockIdx.x * static_cast<uint64_t>(kRowThreads) + threadIdx.x) / kLanes;
   const uint32_t lane = threadIdx.x % kLanes;
   const bool on = i < places;
@@ -395,12 +556,6 @@ uint64_t stride_or(size_t stride, size_t dim, const char* what) {
   return stride ? stride : dim;
 }
 
-void require(const void* p, size_t align, const char* what) {
-  HKV_REQUIRE(p != nullptr, HKV_ERR_INVALID, std::string(what) + " is null");
-  HKV_REQUIRE(reinterpret_cast<uintptr_t>(p) % align == 0, HKV_ERR_INVALID,
-              std::string(what) + " is not aligned to its elements");
-}
-
 // largest word (16 bytes at most) that addresses, strides and rows are
 // multiples of
 uint32_t word_bytes(std::initializer_list<const void*> ptrs, std::initializer_list<uint64_t> sizes) {
@@ -427,12 +582,11 @@ void launch_dispatch(const RowShape& r, const void* x, uint64_t x_stride,
                      uint64_t rows_stride, cudaStream_t s) {
   const uint32_t words = static_cast<uint32_t>(r.dim * r.bytes / kBytes);
   in_slices(r.n, words, [&](size_t t, size_t m) {
-    dispatch_kernel<kBytes><<<blocks_for(m * words), kRowThreads, 0, counted(s)>>>(
-        static_cast<uint32_t>(m * words), FastDiv(words), static_cast<uint32_t>(r.slots),
-        static_cast<const uint8_t*>(x) + t * x_stride * r.bytes, x_stride * r.bytes / kBytes,
-        positions + t * r.slots, static_cast<uint32_t>(num_rows), rows,
-        rows_stride * r.bytes / kBytes);
-    CUDA_TRY(cudaGetLastError());
+    launch(dispatch_kernel<kBytes>, blocks_for(m * words), kRowThreads, 0, s, 1,
+           static_cast<uint32_t>(m * words), FastDiv(words), static_cast<uint32_t>(r.slots),
+           static_cast<const uint8_t*>(x) + t * x_stride * r.bytes, x_stride * r.bytes / kBytes,
+           positions + t * r.slots, static_cast<uint32_t>(num_rows), rows,
+           rows_stride * r.bytes / kBytes);
   });
 }
 
@@ -445,13 +599,12 @@ void launch_combine(const RowShape& r, const void* rows, uint64_t rows_stride, s
     // without positions the rows go by place: those of the slice begin at t * slots
     const size_t skip = positions ? 0 : t * r.slots;
     if (skip > num_rows) num_rows = skip;
-    combine_kernel<T, W, kVec><<<blocks_for(m * packs), kRowThreads, 0, counted(s)>>>(
-        static_cast<uint32_t>(m * packs), FastDiv(packs), static_cast<uint32_t>(r.slots),
-        static_cast<const T*>(rows) + skip * rows_stride, rows_stride,
-        static_cast<uint32_t>(num_rows - skip), positions ? positions + t * r.slots : nullptr,
-        weights ? static_cast<const W*>(weights) + t * r.slots : nullptr,
-        static_cast<T*>(out) + t * out_stride, out_stride);
-    CUDA_TRY(cudaGetLastError());
+    launch(combine_kernel<T, W, kVec>, blocks_for(m * packs), kRowThreads, 0, s, 1,
+           static_cast<uint32_t>(m * packs), FastDiv(packs), static_cast<uint32_t>(r.slots),
+           static_cast<const T*>(rows) + skip * rows_stride, rows_stride,
+           static_cast<uint32_t>(num_rows - skip), positions ? positions + t * r.slots : nullptr,
+           weights ? static_cast<const W*>(weights) + t * r.slots : nullptr,
+           static_cast<T*>(out) + t * out_stride, out_stride);
   });
 }
 
@@ -461,14 +614,12 @@ void launch_backward(const RowShape& r, const void* rows, uint64_t rows_stride, 
                      uint64_t grad_out_stride, void* grad_rows, uint64_t grad_rows_stride,
                      void* grad_weights, cudaStream_t s) {
   const size_t places = r.n * r.slots;
-  combine_backward_kernel<T, W, kVec, kLanes>
-      <<<blocks_for(places * kLanes), kRowThreads, 0, counted(s)>>>(
-          static_cast<uint32_t>(places), FastDiv(static_cast<uint32_t>(r.slots)),
-          static_cast<uint32_t>(r.dim / kVec), static_cast<const T*>(rows), rows_stride,
-          static_cast<uint32_t>(num_rows), positions, static_cast<const W*>(weights),
-          static_cast<const T*>(grad_out), grad_out_stride, static_cast<T*>(grad_rows),
-          grad_rows_stride, static_cast<W*>(grad_weights));
-  CUDA_TRY(cudaGetLastError());
+  launch(combine_backward_kernel<T, W, kVec, kLanes>, blocks_for(places * kLanes), kRowThreads, 0,
+         s, 1, static_cast<uint32_t>(places), FastDiv(static_cast<uint32_t>(r.slots)),
+         static_cast<uint32_t>(r.dim / kVec), static_cast<const T*>(rows), rows_stride,
+         static_cast<uint32_t>(num_rows), positions, static_cast<const W*>(weights),
+         static_cast<const T*>(grad_out), grad_out_stride, static_cast<T*>(grad_rows),
+         grad_rows_stride, static_cast<W*>(grad_weights));
 }
 
 // calls f with the row type and the weight type as values of those types
@@ -505,21 +656,6 @@ int check_combine_types(int value_type, const void* weights, const void* grad_we
 // ===========================================================================
 // C ABI
 // ===========================================================================
-using hkvb::HkvError;
-
-#define HKV_API_BEGIN try {
-#define HKV_API_END                     \
-  return HKV_OK;                        \
-  }                                     \
-  catch (const HkvError& e) {           \
-    hkvb::set_last_error(e.msg);        \
-    return e.code;                      \
-  }                                     \
-  catch (const std::exception& e) {     \
-    hkvb::set_last_error(e.what());     \
-    return HKV_ERR_RUNTIME;             \
-  }
-
 extern "C" {
 
 int hkv_group_workspace(size_t n, uint32_t num_groups, size_t* out_bytes) {
@@ -528,7 +664,7 @@ int hkv_group_workspace(size_t n, uint32_t num_groups, size_t* out_bytes) {
   HKV_REQUIRE(n <= hkvb::kMaxCount, HKV_ERR_INVALID, "n must be below 2^31");
   HKV_REQUIRE(num_groups > 0 && num_groups <= HKV_MAX_GROUPS, HKV_ERR_INVALID,
               "num_groups must be 1 to 4096");
-  *out_bytes = hkvb::sort_workspace(n, num_groups);
+  *out_bytes = hkvb::sort_plan(n, num_groups).workspace;
   HKV_API_END
 }
 
@@ -548,7 +684,7 @@ int hkv_group_tokens(size_t n, const void* groups, int id_type, uint32_t num_gro
     if (order) hkvb::require(order, 4, "order");
   }
   hkvb::require(workspace, 16, "workspace");
-  HKV_REQUIRE(workspace_bytes >= hkvb::sort_workspace(n, num_groups), HKV_ERR_INVALID,
+  HKV_REQUIRE(workspace_bytes >= hkvb::sort_plan(n, num_groups).workspace, HKV_ERR_INVALID,
               "the workspace is smaller than hkv_group_workspace asks for");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (id_type == HKV_ID_I32)
