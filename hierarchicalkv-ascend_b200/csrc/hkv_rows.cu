@@ -14,6 +14,18 @@
 
 #include "hkv_ops.cuh"
 
+#ifndef LD_CS
+#define LD_CS 1
+#endif
+#ifndef ST_CS
+#define ST_CS 1
+#endif
+#ifndef FW_AHEAD
+#define FW_AHEAD 4
+#endif
+#ifndef BW_AHEAD
+#define BW_AHEAD 4
+#endif
 namespace hkvb {
 
 namespace {
@@ -37,10 +49,10 @@ struct FastDiv {
 
 // ---- sort by group ----------------------------------------------------------
 // A counting sort that keeps the order of equal ids. A warp takes a run of
-// 32 * kItems places; __match_any_sync ranks each place among the equal ids of
-// its warp step, the warp's own count of the id among the steps before. The
-// warps' counts, scanned over the warps, and the start of the group in this
-// block's part make the row.
+// 32 * kItems places; ballots over the bits of the ids rank each place among
+// the equal ids of its warp step, the warp's own count of the id among the steps
+// before. The warps' counts, scanned over the warps, and the start of the group
+// in this block's part make the row.
 //
 // Two forms, chosen by n and num_groups (see sort_plan): one launch of one
 // cluster, whose blocks exchange their counts through distributed shared
@@ -54,14 +66,30 @@ __device__ __forceinline__ int load_group(const void* groups, uint64_t i, uint64
   return id >= 0 && id < static_cast<Id>(num_groups) ? static_cast<int>(id) : -1;
 }
 
+// Lanes of the warp with the same id, by one ballot per bit of an id XX. Of no meaning for a lane without one.
+__device__ __forceinline__ uint32_t same_id(int id, uint32_t bits) {
+  uint32_t same = __ballot_sync(~0u, id >= 0);
+#pragma unroll 4
+  for (uint32_t b = 0; b < bits; b++) {
+    const bool on = id >> b & 1;
+    const uint32_t lanes = __ballot_sync(~0u, on);
+    same &= on ? lanes : ~lanes;
+  }
+  return same;
+}
+
+__device__ __forceinline__ uint32_t id_bits(uint32_t num_groups) {
+  return 32 - __clz(num_groups - 1);  // 0 for one group
+}
+
 // Ranks of a warp's places; mine[g] counts the warp's places of group g.
 template <int kItems>
 __device__ __forceinline__ void rank_in_warp(const int (&id)[kItems], uint16_t* mine,
-                                             uint32_t (&rank)[kItems]) {
+                                             uint32_t bits, uint32_t (&rank)[kItems]) {
   const uint32_t below = (1u << (threadIdx.x & 31)) - 1;
 #pragma unroll
   for (int it = 0; it < kItems; it++) {
-    const uint32_t same = __match_any_sync(~0u, id[it]);
+    const uint32_t same = same_id(id[it], bits);
     const uint32_t before = id[it] >= 0 ? mine[id[it]] : 0;
     rank[it] = before + __popc(same & below);
     __syncwarp();
@@ -128,7 +156,7 @@ __global__ void __launch_bounds__(kClusterThreads)
   for (int it = 0; it < kItems; it++) id[it] = load_group<Id>(groups, base + it * 32, n, num_groups);
   __syncthreads();
   uint16_t* mine = cnt + warp * num_groups;
-  rank_in_warp(id, mine, rank);
+  rank_in_warp(id, mine, id_bits(num_groups), rank);
   __syncthreads();
   for (uint32_t g = threadIdx.x; g < num_groups; g += threads)
     mine_all[g] = scan_over_warps(cnt, warps, num_groups, g);
@@ -199,7 +227,7 @@ __global__ void __launch_bounds__(kSortThreads)
   constexpr uint64_t kTile = kSortThreads * kItems;
   const uint64_t first = static_cast<uint64_t>(blockIdx.x) * tiles_per_block * kTile;
   const uint64_t last = min(n, first + tiles_per_block * kTile);
-  const uint32_t below = (1u << (threadIdx.x & 31)) - 1;
+  const uint32_t below = (1u << (threadIdx.x & 31)) - 1, bits = id_bits(num_groups);
   for (uint64_t base = first; base < last; base += kTile) {
     int id[kItems];
 #pragma unroll
@@ -207,7 +235,7 @@ __global__ void __launch_bounds__(kSortThreads)
       id[it] = load_group<Id>(groups, base + it * kSortThreads + threadIdx.x, last, num_groups);
 #pragma unroll
     for (int it = 0; it < kItems; it++) {
-      const uint32_t same = __match_any_sync(~0u, id[it]);
+      const uint32_t same = same_id(id[it], bits);
       if (id[it] >= 0 && (same & below) == 0) atomicAdd(&hist[id[it]], __popc(same));
     }
   }
@@ -282,7 +310,7 @@ __global__ void __launch_bounds__(kSortThreads)
     for (uint32_t k = threadIdx.x; k < num_groups * kSortWarps; k += kSortThreads) cnt[k] = 0;
     __syncthreads();
     uint16_t* mine = cnt + warp * num_groups;
-    rank_in_warp(id, mine, rank);
+    rank_in_warp(id, mine, id_bits(num_groups), rank);
     __syncthreads();
     for (uint32_t g = threadIdx.x; g < num_groups; g += kSortThreads)
       cnt[kSortWarps * num_groups + g] = scan_over_warps(cnt, kSortWarps, num_groups, g);
@@ -317,12 +345,18 @@ size_t cluster_smem(uint32_t num_groups, uint32_t threads, uint32_t items) {
          static_cast<size_t>(num_groups) * (threads / 32) * 2;
 }
 
+// Places of the one-launch form: 8 blocks of 1024 threads, four places each.
+// Measured (us a sort in a graph, 64 groups, one launch against three): 128
+// places 2.0 / 5.1, 4096 5.0 / 5.3, 16384 5.4 / 5.9, 32768 7.3 / 5.9, 131072
+// 16.6 / 7.2. The two further launches cost 4 us of host time where the host
+// is what a pass waits for, so the border is above the crossing.
 constexpr uint32_t kMaxCluster = 8;
+constexpr uint32_t kClusterItems = 4;
 
 SortPlan sort_plan(size_t n, uint32_t num_groups) {
   SortPlan p{};
   // one launch while a block's share fits its registers and shared memory
-  if (n <= static_cast<size_t>(kMaxCluster) * kClusterThreads * 16) {
+  if (n <= static_cast<size_t>(kMaxCluster) * kClusterThreads * kClusterItems) {
     const uint32_t m = std::max<uint32_t>(1, static_cast<uint32_t>(n));
     p.blocks = 1;
     while (p.blocks < kMaxCluster && m > p.blocks * kClusterThreads * 2) p.blocks *= 2;
@@ -357,8 +391,7 @@ void with_items(uint32_t items, F f) {
     case 1: f(std::integral_constant<int, 1>{}); break;
     case 2: f(std::integral_constant<int, 2>{}); break;
     case 4: f(std::integral_constant<int, 4>{}); break;
-    case 8: f(std::integral_constant<int, 8>{}); break;
-    default: f(std::integral_constant<int, 16>{});
+    default: f(std::integral_constant<int, 8>{});
   }
 }
 
@@ -376,26 +409,26 @@ void launch_sort(size_t n, const void* groups, uint32_t num_groups, int32_t* off
   with_items(p.items, [&](auto items) {
     constexpr int kItems = decltype(items)::value;
     if (p.cluster) {
-      auto kernel = group_cluster_kernel<Id, kItems>;
-      allow_smem(kernel, p.smem);
-      launch(kernel, p.blocks, p.threads, p.smem, s, p.blocks, static_cast<uint32_t>(n), groups,
-             num_groups, p.blocks, offsets, positions, order);
+      if constexpr (kItems <= static_cast<int>(kClusterItems)) {
+        auto kernel = group_cluster_kernel<Id, kItems>;
+        allow_smem(kernel, p.smem);
+        launch(kernel, p.blocks, p.threads, p.smem, s, p.blocks, static_cast<uint32_t>(n), groups,
+               num_groups, p.blocks, offsets, positions, order);
+      }
       return;
     }
-    if constexpr (kItems <= 8) {
-      uint32_t* counts = static_cast<uint32_t*>(workspace);
-      uint32_t* totals = counts + static_cast<size_t>(num_groups) * p.blocks;
-      const uint64_t n64 = n;
-      launch(group_count_kernel<Id, kItems>, p.blocks, kSortThreads, num_groups * 4, s, 1, n64,
-             groups, num_groups, p.run, counts);
-      launch(group_scan_kernel, (num_groups + 7) / 8, 256, 0, s, 1, num_groups, p.blocks, counts,
-             totals);
-      auto kernel = group_place_kernel<Id, kItems>;
-      allow_smem(kernel, p.smem);
-      launch(kernel, p.blocks, kSortThreads, p.smem, s, 1, n64, groups, num_groups, p.run,
-             static_cast<const uint32_t*>(counts), static_cast<const uint32_t*>(totals), offsets,
-             positions, order);
-    }
+    uint32_t* counts = static_cast<uint32_t*>(workspace);
+    uint32_t* totals = counts + static_cast<size_t>(num_groups) * p.blocks;
+    const uint64_t n64 = n;
+    launch(group_count_kernel<Id, kItems>, p.blocks, kSortThreads, num_groups * 4, s, 1, n64,
+           groups, num_groups, p.run, counts);
+    launch(group_scan_kernel, (num_groups + 7) / 8, 256, 0, s, 1, num_groups, p.blocks, counts,
+           totals);
+    auto kernel = group_place_kernel<Id, kItems>;
+    allow_smem(kernel, p.smem);
+    launch(kernel, p.blocks, kSortThreads, p.smem, s, 1, n64, groups, num_groups, p.run,
+           static_cast<const uint32_t*>(counts), static_cast<const uint32_t*>(totals), offsets,
+           positions, order);
   });
 }
 
@@ -450,12 +483,34 @@ struct alignas(sizeof(T) * kVec) Pack {
   T v[kVec];
 };
 
-// A thread sums one pack of a token's output over its slots.
+// Rows are read and written once: they need not stay in the caches.
+template <class P>
+__device__ __forceinline__ P load_once(const void* p) {
+  if constexpr (sizeof(P) == 16 && LD_CS) {
+    const uint4 u = __ldcs(static_cast<const uint4*>(p));
+    return reinterpret_cast<const P&>(u);
+  } else {
+    return *static_cast<const P*>(p);
+  }
+}
+template <class P>
+__device__ __forceinline__ void store_once(void* p, const P& v) {
+  if constexpr (sizeof(P) == 16 && ST_CS)
+    __stcs(static_cast<uint4*>(p), reinterpret_cast<const uint4&>(v));
+  else
+    *static_cast<P*>(p) = v;
+}
+
+// A thread sums one pack of a token's output over its slots, kAhead rows in
+// flight at a time.
 template <class T, class W, int kVec>
 __global__ void __launch_bounds__(kRowThreads)
-    combine_kernel(uint32_t packs_of_all, FastDiv packs, uint32_t slots, const T* rows,
-                   uint64_t rows_stride, uint32_t num_rows, const int32_t* positions,
-                   const W* weights, T* out, uint64_t out_stride) {
+    combine_kernel(uint32_t packs_of_all, FastDiv packs, uint32_t slots,
+                   const T* __restrict__ rows, uint64_t rows_stride, uint32_t num_rows,
+                   const int32_t* __restrict__ positions, const W* __restrict__ weights,
+                   T* __restrict__ out, uint64_t out_stride) {
+  using P = Pack<T, kVec>;
+  constexpr int kAhead = FW_AHEAD;
   after_previous();
   const uint32_t i = blockIdx.x * kRowThreads + threadIdx.x;
   if (i >= packs_of_all) return;
@@ -464,60 +519,119 @@ __global__ void __launch_bounds__(kRowThreads)
   float acc[kVec];
 #pragma unroll
   for (int e = 0; e < kVec; e++) acc[e] = 0.f;
-  for (uint32_t k = 0; k < slots; k++) {
-    const uint32_t row = positions ? static_cast<uint32_t>(positions[place + k])
-                                   : static_cast<uint32_t>(place + k);
-    if (row >= num_rows) continue;
-    const float w = weights ? to_float(weights[place + k]) : 1.f;
-    const auto v = *reinterpret_cast<const Pack<T, kVec>*>(rows + row * rows_stride + c);
+  for (uint32_t k = 0; k < slots; k += kAhead) {
+    uint32_t row[kAhead];
+    float w[kAhead];
+    P v[kAhead];
 #pragma unroll
-    for (int e = 0; e < kVec; e++) acc[e] = fmaf(w, to_float(v.v[e]), acc[e]);
+    for (int a = 0; a < kAhead; a++)
+      row[a] = k + a >= slots ? ~0u
+               : positions    ? static_cast<uint32_t>(positions[place + k + a])
+                              : static_cast<uint32_t>(place + k + a);
+#pragma unroll
+    for (int a = 0; a < kAhead; a++)
+      if (row[a] < num_rows) v[a] = load_once<P>(rows + row[a] * rows_stride + c);
+#pragma unroll
+    for (int a = 0; a < kAhead; a++)
+      w[a] = weights && row[a] < num_rows ? to_float(weights[place + k + a]) : 1.f;
+#pragma unroll
+    for (int a = 0; a < kAhead; a++)
+      if (row[a] < num_rows) {
+#pragma unroll
+        for (int e = 0; e < kVec; e++) acc[e] = fmaf(w[a], to_float(v[a].v[e]), acc[e]);
+      }
   }
-  Pack<T, kVec> o;
+  P o;
 #pragma unroll
   for (int e = 0; e < kVec; e++) o.v[e] = from_float<T>(acc[e]);
-  *reinterpret_cast<Pack<T, kVec>*>(out + t * out_stride + c) = o;
+  store_once(out + t * out_stride + c, o);
 }
 
-// kLanes lanes per place: the row of the gradient, and the inner product in
-// per-lane sums joined by a fixed tree of shuffles.
-template <class T, class W, int kVec, int kLanes>
-__global__ void __launch_bounds__(kRowThreads)
-    combine_backward_kernel(uint32_t places, FastDiv slots, uint32_t packs, const T* rows,
-                            uint64_t rows_stride, uint32_t num_rows, const int32_t* positions,
-                            const W* weights, const T* grad_out, uint64_t grad_out_stride,
-                            T* grad_rows, uint64_t grad_rows_stride, W* grad_weights) {
+// kTeam threads per token hold a pack of its gradient at a time and go over its
+// slots, kAhead rows in flight: the rows' gradients, and the inner products in
+// per-thread sums joined by a fixed tree of shuffles (and, for teams of several
+// warps, through shared memory).
+#ifndef BW_BLOCKS
+#define BW_BLOCKS 1
+#endif
+template <class T, class W, int kVec, int kTeam>
+__global__ void __launch_bounds__(kRowThreads, BW_BLOCKS)
+    combine_backward_kernel(uint32_t n, uint32_t slots, uint32_t packs,
+                            const T* __restrict__ rows, uint64_t rows_stride, uint32_t num_rows,
+                            const int32_t* __restrict__ positions, const W* __restrict__ weights,
+                            const T* __restrict__ grad_out, uint64_t grad_out_stride,
+                            T* __restrict__ grad_rows, uint64_t grad_rows_stride,
+                            W* __restrict__ grad_weights) {
+  using P = Pack<T, kVec>;
+  constexpr int kAhead = BW_AHEAD, kWarps = kTeam / 32;
+  __shared__ float sums[2][kAhead][kRowThreads / 32];
   after_previous();
-  const uint32_t i = (blockIdx.x * static_cast<uint64_t>(kRowThreads) + threadIdx.x) / kLanes;
-  const uint32_t lane = threadIdx.x % kLanes;
-  const bool on = i < places;
-  const uint32_t row = !on ? ~0u : positions ? static_cast<uint32_t>(positions[i]) : i;
-  const bool has = row < num_rows;
-  float dot = 0.f;
-  if (has) {
-    const float w = weights ? to_float(weights[i]) : 1.f;
-    const T* g = grad_out + slots.div(i) * grad_out_stride;
-    const T* y = rows + row * rows_stride;
-    T* gy = grad_rows + row * grad_rows_stride;
-    for (uint32_t p = lane; p < packs; p += kLanes) {
-      const auto gv = *reinterpret_cast<const Pack<T, kVec>*>(g + p * kVec);
+  const uint32_t t = (blockIdx.x * static_cast<uint64_t>(kRowThreads) + threadIdx.x) / kTeam;
+  const uint32_t lane = threadIdx.x % kTeam;
+  const uint64_t place = static_cast<uint64_t>(t) * slots;
+  const T* g = grad_out + t * grad_out_stride;
+  for (uint32_t k = 0; k < slots; k += kAhead) {
+    uint32_t row[kAhead];
+    float w[kAhead], dot[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; a++) {
+      const bool on = t < n && k + a < slots;
+      row[a] = !on         ? ~0u
+               : positions ? static_cast<uint32_t>(positions[place + k + a])
+                           : static_cast<uint32_t>(place + k + a);
+      w[a] = weights && row[a] < num_rows ? to_float(weights[place + k + a]) : 1.f;
+      dot[a] = 0.f;
+    }
+    for (uint32_t p = lane; t < n && p < packs; p += kTeam) {
+      const P gv = *reinterpret_cast<const P*>(g + p * kVec);
+      P yv[kAhead];
       if (grad_weights) {
-        const auto yv = *reinterpret_cast<const Pack<T, kVec>*>(y + p * kVec);
 #pragma unroll
-        for (int e = 0; e < kVec; e++) dot = fmaf(to_float(gv.v[e]), to_float(yv.v[e]), dot);
+        for (int a = 0; a < kAhead; a++)
+          if (row[a] < num_rows) yv[a] = load_once<P>(rows + row[a] * rows_stride + p * kVec);
       }
-      if (grad_rows) {
-        Pack<T, kVec> o;
 #pragma unroll
-        for (int e = 0; e < kVec; e++) o.v[e] = from_float<T>(w * to_float(gv.v[e]));
-        *reinterpret_cast<Pack<T, kVec>*>(gy + p * kVec) = o;
+      for (int a = 0; a < kAhead; a++) {
+        if (row[a] >= num_rows) continue;
+        if (grad_rows) {
+          P o;
+#pragma unroll
+          for (int e = 0; e < kVec; e++) o.v[e] = from_float<T>(w[a] * to_float(gv.v[e]));
+          store_once(grad_rows + row[a] * grad_rows_stride + p * kVec, o);
+        }
+        if (grad_weights) {
+#pragma unroll
+          for (int e = 0; e < kVec; e++)
+            dot[a] = fmaf(to_float(gv.v[e]), to_float(yv[a].v[e]), dot[a]);
+        }
       }
     }
-  }
-  if (grad_weights) {
+    if (!grad_weights) continue;
 #pragma unroll
-    for (int o = kLanes / 2; o; o >>= 1) dot += __shfl_xor_sync(~0u, dot, o, kLanes);
-    if (on && lane == 0) grad_weights[i] = from_float<W>(dot);
+    for (int a = 0; a < kAhead; a++) {
+#pragma unroll
+      for (int o = (kTeam < 32 ? kTeam : 32) / 2; o; o >>= 1)
+        dot[a] += __shfl_xor_sync(~0u, dot[a], o);
+    }
+    if constexpr (kTeam > 32) {
+      float(*const s)[kRowThreads / 32] = sums[k / kAhead & 1];
+      if (lane % 32 == 0) {
+#pragma unroll
+        for (int a = 0; a < kAhead; a++) s[a][threadIdx.x / 32] = dot[a];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int a = 0; a < kAhead; a++) {
+        dot[a] = 0.f;
+#pragma unroll
+        for (int v = 0; v < kWarps; v++) dot[a] += s[a][threadIdx.x / kTeam * kWarps + v];
+      }
+    }
+    if (t < n && lane == 0) {
+#pragma unroll
+      for (int a = 0; a < kAhead; a++)
+        if (k + a < slots) grad_weights[place + k + a] = from_float<W>(dot[a]);
+    }
   }
 }
 
@@ -608,14 +722,13 @@ void launch_combine(const RowShape& r, const void* rows, uint64_t rows_stride, s
   });
 }
 
-template <class T, class W, int kVec, int kLanes>
+template <class T, class W, int kVec, int kTeam>
 void launch_backward(const RowShape& r, const void* rows, uint64_t rows_stride, size_t num_rows,
                      const int32_t* positions, const void* weights, const void* grad_out,
                      uint64_t grad_out_stride, void* grad_rows, uint64_t grad_rows_stride,
                      void* grad_weights, cudaStream_t s) {
-  const size_t places = r.n * r.slots;
-  launch(combine_backward_kernel<T, W, kVec, kLanes>, blocks_for(places * kLanes), kRowThreads, 0,
-         s, 1, static_cast<uint32_t>(places), FastDiv(static_cast<uint32_t>(r.slots)),
+  launch(combine_backward_kernel<T, W, kVec, kTeam>, blocks_for(r.n * kTeam), kRowThreads, 0, s, 1,
+         static_cast<uint32_t>(r.n), static_cast<uint32_t>(r.slots),
          static_cast<uint32_t>(r.dim / kVec), static_cast<const T*>(rows), rows_stride,
          static_cast<uint32_t>(num_rows), positions, static_cast<const W*>(weights),
          static_cast<const T*>(grad_out), grad_out_stride, static_cast<T*>(grad_rows),
@@ -772,17 +885,21 @@ int hkv_combine_rows_backward(size_t n, size_t slots, size_t dim, int value_type
     using T = decltype(t);
     using W = decltype(w);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    auto go = [&](auto vec, auto lanes) {
-      hkvb::launch_backward<T, W, decltype(vec)::value, decltype(lanes)::value>(
+    auto go = [&](auto vec, auto team) {
+      hkvb::launch_backward<T, W, decltype(vec)::value, decltype(team)::value>(
           r, rows, rs, num_rows, positions, weights, grad_out, gs, grad_rows, ys, grad_weights,
           s);
     };
-    auto pick = [&](auto vec) {
+    auto pick = [&](auto vec) {  // the smallest team that covers a row, 256 at most
       const size_t packs = dim / decltype(vec)::value;
       if (packs <= 8)
         go(vec, std::integral_constant<int, 8>{});
-      else
+      else if (packs <= 32)
         go(vec, std::integral_constant<int, 32>{});
+      else if (packs <= 128)
+        go(vec, std::integral_constant<int, 128>{});
+      else
+        go(vec, std::integral_constant<int, 256>{});
     };
     if (wide)
       pick(std::integral_constant<int, 16 / sizeof(T)>{});
