@@ -42,29 +42,64 @@ __device__ __forceinline__ void after_previous() {
   cudaTriggerProgrammaticLaunchCompletion();  // the next one may be set up
 }
 
-// Exclusive sum of v over the threads of a block, and the sum of all.
-__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* total) {
-  __shared__ uint32_t sums[32];
+// Blocks of a cluster. The barrier orders shared and global memory among them.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n"
+               "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// word `p` of this block's shared memory, in block `rank` of the cluster
+__device__ __forceinline__ uint32_t load_remote(const uint32_t* p, uint32_t rank) {
+  uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(p)), r, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(r) : "memory");
+  return v;
+}
+
+// Exclusive sums of two values over the threads of a block, and the sums of all.
+__device__ __forceinline__ void block_exclusive2(uint32_t v, uint32_t u, uint32_t* v_before,
+                                                 uint32_t* u_before, uint32_t* v_all,
+                                                 uint32_t* u_all) {
+  __shared__ uint2 sums[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  uint32_t inc = v;
+  uint32_t a = v, b = u;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t u = __shfl_up_sync(~0u, inc, o);
-    if (lane >= o) inc += u;
+    const uint32_t x = __shfl_up_sync(~0u, a, o), y = __shfl_up_sync(~0u, b, o);
+    if (lane >= o) {
+      a += x;
+      b += y;
+    }
   }
   __syncthreads();  // the sums of a call before are read
-  if (lane == 31) sums[warp] = inc;
+  if (lane == 31) sums[warp] = make_uint2(a, b);
   __syncthreads();
   // every warp scans the warps' sums for itself
-  uint32_t w = lane < warps ? sums[lane] : 0;
+  uint2 w = lane < warps ? sums[lane] : make_uint2(0, 0);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t u = __shfl_up_sync(~0u, w, o);
-    if (lane >= o) w += u;
+    const uint32_t x = __shfl_up_sync(~0u, w.x, o), y = __shfl_up_sync(~0u, w.y, o);
+    if (lane >= o) {
+      w.x += x;
+      w.y += y;
+    }
   }
-  *total = __shfl_sync(~0u, w, 31);
-  const uint32_t before = __shfl_sync(~0u, w, warp ? warp - 1 : 0);
-  return (warp ? before : 0) + inc - v;
+  *v_all = __shfl_sync(~0u, w.x, 31);
+  *u_all = __shfl_sync(~0u, w.y, 31);
+  const uint32_t x = __shfl_sync(~0u, w.x, warp ? warp - 1 : 0);
+  const uint32_t y = __shfl_sync(~0u, w.y, warp ? warp - 1 : 0);
+  *v_before = (warp ? x : 0) + a - v;
+  *u_before = (warp ? y : 0) + b - u;
+}
+
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* total) {
+  uint32_t before, zero, none;
+  block_exclusive2(v, 0, &before, &zero, total, &none);
+  return before;
 }
 
 // A non-null address that is a multiple of its elements' size.

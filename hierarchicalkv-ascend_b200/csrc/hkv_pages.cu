@@ -54,10 +54,11 @@ template <> struct Word<16> { using type = uint4; };
 template <> struct Word<4> { using type = uint32_t; };
 template <> struct Word<1> { using type = uint8_t; };
 
-// Moves chunk c (0 <= c < planes.chunks) of page src to page dst.
+// Moves chunk c (0 <= c < planes.chunks) of page src to page dst; the work of
+// thread tid of kCopyThreads.
 template <int kBytes>
 __device__ __forceinline__ void copy_chunk(const PlaneSet& planes, uint32_t c, uint32_t src,
-                                           uint32_t dst) {
+                                           uint32_t dst, uint32_t tid) {
   using T = typename Word<kBytes>::type;
   uint32_t lo = 0, hi = planes.num - 1;  // last plane that begins at or before c
   while (lo < hi) {
@@ -71,7 +72,7 @@ __device__ __forceinline__ void copy_chunk(const PlaneSet& planes, uint32_t c, u
   const T* from = reinterpret_cast<const T*>(p.base) + src * p.page_words;
   T* to = reinterpret_cast<T*>(p.base) + dst * p.page_words;
   const uint64_t first =
-      static_cast<uint64_t>(c - p.first_chunk) * kCopyThreads * kCopyUnroll + threadIdx.x;
+      static_cast<uint64_t>(c - p.first_chunk) * kCopyThreads * kCopyUnroll + tid;
   T v[kCopyUnroll];
 #pragma unroll
   for (uint32_t u = 0; u < kCopyUnroll; u++)
@@ -90,8 +91,85 @@ __global__ void __launch_bounds__(kCopyThreads)
   const uint32_t pair = blockIdx.x / planes.chunks, c = blockIdx.x - pair * planes.chunks;
   const uint32_t s = static_cast<uint32_t>(src[pair]), d = static_cast<uint32_t>(dst[pair]);
   if (s >= num_pages || d >= num_pages || s == d) return;
-  copy_chunk<kBytes>(planes, c, s, d);
+  copy_chunk<kBytes>(planes, c, s, d, threadIdx.x);
 }
+
+// ---- fork -------------------------------------------------------------------
+// Every source is read before any row is written, since a row may be source and
+// destination. Entry j of a row depends on entries j of other rows only, so a
+// block that takes kForkColumns columns of the whole list needs no other block:
+// it reads its sources and what its destinations held (counts + 1 and - 1), then
+// writes. Lengths are read by all blocks and written by the last one to have
+// read them. The sums of counts do not depend on the order of their atomics.
+
+constexpr uint32_t kForkColumns = 8;  // a sector of a row
+constexpr uint32_t kForkColumnThreads = 1024;
+
+struct ForkEntry {
+  int32_t src, dst;
+  int32_t length;  // new length, -1: entry passed over
+  int32_t old;     // length of the destination before
+};
+
+__global__ void __launch_bounds__(kForkColumnThreads)
+    fork_columns_kernel(PoolView v, uint32_t n, const int32_t* src, const int32_t* dst,
+                        uint32_t* arrived) {
+  extern __shared__ int4 fork_smem_[];
+  ForkEntry* entry = reinterpret_cast<ForkEntry*>(fork_smem_);  // [n]
+  int32_t* staged = reinterpret_cast<int32_t*>(entry + n);      // [n][kForkColumns]
+  int32_t* owner = staged + n * kForkColumns;  // [num_rows] last entry of each destination
+  __shared__ bool last;
+  for (uint32_t r = threadIdx.x; r < v.num_rows; r += kForkColumnThreads) owner[r] = -1;
+  after_previous();
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < n; e += kForkColumnThreads) {
+    ForkEntry f{src[e], dst[e], -1, 0};
+    const bool to = static_cast<uint32_t>(f.dst) < v.num_rows;
+    if (to) atomicMax(&owner[f.dst], static_cast<int32_t>(e));
+    if (to && static_cast<uint32_t>(f.src) < v.num_rows) {
+      f.length = max(0, v.lengths[f.src]);
+      f.old = max(0, v.lengths[f.dst]);
+    }
+    entry[e] = f;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(arrived, 1u) == gridDim.x - 1;
+  }
+  const uint32_t j0 = blockIdx.x * kForkColumns;
+  for (uint32_t k = threadIdx.x; k < n * kForkColumns; k += kForkColumnThreads) {
+    const uint32_t e = k / kForkColumns, j = j0 + k % kForkColumns;
+    const ForkEntry f = entry[e];
+    if (f.length < 0 || owner[f.dst] != static_cast<int32_t>(e)) continue;
+    const bool now = j < v.pages_of(f.length), before = j < v.pages_of(f.old);
+    const int32_t page = now ? v.row(f.src)[j] : -1, held = before ? v.row(f.dst)[j] : -1;
+    staged[k] = page;
+    if (static_cast<uint32_t>(page) < v.num_pages) atomicAdd(&v.refs[page], 1);
+    if (static_cast<uint32_t>(held) < v.num_pages) atomicSub(&v.refs[held], 1);
+  }
+  __syncthreads();
+  for (uint32_t k = threadIdx.x; k < n * kForkColumns; k += kForkColumnThreads) {
+    const uint32_t e = k / kForkColumns, j = j0 + k % kForkColumns;
+    const ForkEntry f = entry[e];
+    if (f.length >= 0 && j < v.pages_of(f.length) && owner[f.dst] == static_cast<int32_t>(e))
+      v.row(f.dst)[j] = staged[k];
+  }
+  if (last) {
+    for (uint32_t e = threadIdx.x; e < n; e += kForkColumnThreads) {
+      const ForkEntry f = entry[e];
+      if (f.length >= 0 && owner[f.dst] == static_cast<int32_t>(e)) v.lengths[f.dst] = f.length;
+    }
+    if (threadIdx.x == 0) *arrived = 0;
+  }
+}
+
+size_t fork_smem(uint32_t num_rows, size_t n) {
+  return n * (sizeof(ForkEntry) + kForkColumns * 4) + num_rows * 4ull;
+}
+
+// Longer lists, and pools beyond the shared memory of a block: the same in two
+// launches, through global memory. Blocks (list entry, chunk of table entries).
 
 // Whether an entry behind e names the same row; asked by a whole block.
 __device__ __forceinline__ bool named_again(const int32_t* rows, uint32_t e, uint32_t n,
@@ -100,12 +178,6 @@ __device__ __forceinline__ bool named_again(const int32_t* rows, uint32_t e, uin
   for (uint32_t k = e + 1 + threadIdx.x; k < n; k += blockDim.x) again |= rows[k] == row;
   return __syncthreads_or(again);
 }
-
-// ---- fork -------------------------------------------------------------------
-// Two launches, since a row may be source and destination: the first reads
-// every source (entries to `staged`, counts + 1), the second writes every
-// destination (counts - 1 for what it held). Blocks (list entry, chunk of table
-// entries); the sums of counts do not depend on the order of their atomics.
 
 constexpr uint32_t kForkThreads = 256;
 constexpr uint32_t kForkChunk = 1024;  // table entries of a block
@@ -201,242 +273,346 @@ __device__ __forceinline__ uint32_t live_bits(int4 c) {
   return (c.x > 0) | (c.y > 0) << 1 | (c.z > 0) << 2 | (c.w > 0) << 3;
 }
 
-// sums of counts[0 .. strip) and of counts[0 .. strips)
-__device__ __forceinline__ void strip_base(const uint32_t* counts, uint32_t strip, uint32_t strips,
-                                           uint32_t* before, uint32_t* all) {
-  uint32_t b = 0, a = 0;
-  for (uint32_t k = threadIdx.x; k < strips; k += blockDim.x) {
-    const uint32_t c = counts[k];
-    a += c;
-    if (k < strip) b += c;
+// The planning of resize and compact is a few dependent passes over small
+// arrays: one cluster of kPlanBlocks blocks does them in one launch, each block
+// on its share, with sums exchanged through distributed shared memory.
+constexpr uint32_t kPlanBlocks = 8;
+
+// strips of a block: [first, last)
+__device__ __forceinline__ void plan_share(uint32_t count, uint32_t rank, uint32_t* first,
+                                           uint32_t* last) {
+  const uint32_t each = (count + kPlanBlocks - 1) / kPlanBlocks;
+  *first = min(count, rank * each);
+  *last = min(count, *first + each);
+}
+
+// Sums of a and b over the blocks before this one and over all. `shared` must
+// not be written again before the cluster's next barrier.
+__device__ __forceinline__ void exchange(uint32_t a, uint32_t b, uint32_t rank, uint32_t* shared,
+                                         uint32_t* a_before, uint32_t* a_all, uint32_t* b_before,
+                                         uint32_t* b_all) {
+  if (threadIdx.x == 0) {
+    shared[0] = a;
+    shared[1] = b;
   }
-  block_exclusive(b, before);
-  block_exclusive(a, all);
+  cluster_sync();
+  // lane k of each warp reads from block k
+  const uint32_t k = threadIdx.x % 32;
+  const uint32_t x = k < kPlanBlocks ? load_remote(shared, k) : 0;
+  const uint32_t y = k < kPlanBlocks ? load_remote(shared + 1, k) : 0;
+  *a_all = __reduce_add_sync(~0u, x);
+  *b_all = __reduce_add_sync(~0u, y);
+  *a_before = __reduce_add_sync(~0u, k < rank ? x : 0);
+  *b_before = __reduce_add_sync(~0u, k < rank ? y : 0);
 }
 
 // ---- resize -----------------------------------------------------------------
-// Three launches: what each entry wants and how many pages of each strip are
-// free; the list of free pages and each entry's place in it; the changes
-// themselves with the page copies.
+// The plan: what each entry wants, the list of free pages as far as it is
+// wanted, each entry's place in it. Then the changes with the page copies, in
+// the same launch where the copies are few, else in a second one.
 
 struct Want {
   int32_t row;     // -1: entry passed over
   int32_t old, length;
   int32_t shared;  // last page to copy, -1: none
+  uint32_t first;  // place in the list of free pages, ~0: not served
 };
-constexpr uint32_t kStripWarps = kStripThreads / 32;
 
-// Blocks 0 to strips - 1 count free pages, the others take a list entry per warp.
-// needs[e]: pages that entry e wants to take.
-__global__ void __launch_bounds__(kStripThreads)
-    resize_count_kernel(PoolView v, uint32_t n, const int32_t* rows, const int32_t* lengths,
-                        uint32_t strips, uint32_t* counts, Want* wants, uint32_t* needs) {
-  after_previous();
-  if (blockIdx.x < strips) {
-    uint32_t first, total;
-    const int4 c = strip_counts(v, blockIdx.x, &first);
-    block_exclusive(__popc(free_bits(c)), &total);
-    if (threadIdx.x == 0) counts[blockIdx.x] = total;
-    return;
-  }
-  const uint32_t e = (blockIdx.x - strips) * kStripWarps + (threadIdx.x >> 5);
-  const uint32_t lane = threadIdx.x & 31;
-  if (e >= n) return;
-  const int32_t r = rows[e];
-  bool again = false;
-  for (uint32_t k = e + 1 + lane; k < n; k += 32) again |= rows[k] == r;
-  again = __any_sync(~0u, again);
-  if (lane != 0) return;
-  Want w{-1, 0, lengths[e], -1};
-  uint32_t need = 0;
-  if (!again && static_cast<uint32_t>(r) < v.num_rows && w.length >= 0 &&
-      static_cast<uint64_t>(w.length) <= static_cast<uint64_t>(v.max_pages) * v.page_tokens) {
-    w.row = r;
-    w.old = max(0, v.lengths[r]);
-    const uint32_t have = v.pages_of(w.old), want = v.pages_of(w.length);
-    if (w.length > w.old && w.old % v.page_tokens != 0) {
-      const int32_t last = v.row(r)[have - 1];
-      if (static_cast<uint32_t>(last) < v.num_pages && v.refs[last] > 1) w.shared = last;
-    }
-    need = (want > have ? want - have : 0) + (w.shared >= 0);
-  }
-  wants[e] = w;
-  needs[e] = need;
-}
-
-__global__ void __launch_bounds__(kStripThreads)
-    resize_list_kernel(PoolView v, uint32_t n, uint32_t strips, const uint32_t* counts,
-                       const uint32_t* needs, uint32_t* first_of, int32_t* free_list) {
-  after_previous();
-  if (blockIdx.x == strips) {  // places in the list, in the entries' order
-    uint32_t free, ignored, run = 0;
-    strip_base(counts, strips, strips, &free, &ignored);
-    for (uint32_t e0 = 0; e0 < n; e0 += kStripThreads) {
-      const uint32_t e = e0 + threadIdx.x;
-      const uint32_t need = e < n ? needs[e] : 0;
-      uint32_t total;
-      const uint32_t first = run + block_exclusive(need, &total);
-      // served: needs nothing, or all that is wanted up to here is there (the
-      // sum stays below 2^32: rows differ, and each wants max_pages + 1 at most)
-      if (e < n) first_of[e] = need == 0 || first + need <= free ? first : ~0u;
-      run += total;
-    }
-    return;
-  }
-  uint32_t wanted = 0, total, before, all;
-  for (uint32_t e = threadIdx.x; e < n; e += kStripThreads) wanted += needs[e];
-  block_exclusive(wanted, &total);
-  if (total == 0) return;
-  strip_base(counts, blockIdx.x, strips, &before, &all);
-  if (before >= total) return;  // earlier strips have enough
-  uint32_t first;
-  const uint32_t bits = free_bits(strip_counts(v, blockIdx.x, &first));
-  uint32_t at = before + block_exclusive(__popc(bits), &all);
-#pragma unroll
-  for (int k = 0; k < 4; k++)
-    if (bits >> k & 1) free_list[at++] = first + k;
-}
-
+// Chunk y of `chunks_at_once` of entry e: the first one also changes the table.
 template <int kBytes>
-__global__ void __launch_bounds__(kCopyThreads)
-    resize_apply_kernel(const __grid_constant__ PlaneSet planes, PoolView v, const Want* wants,
-                        const uint32_t* first_of, const int32_t* free_list, bool* status) {
-  after_previous();
-  const uint32_t e = blockIdx.x;
+__device__ __forceinline__ void resize_entry(const PlaneSet& planes, const PoolView& v,
+                                             const Want* wants, const int32_t* free_list,
+                                             bool* status, uint32_t e, uint32_t y,
+                                             uint32_t chunks_at_once, uint32_t tid) {
   const Want w = wants[e];
-  const uint32_t first = first_of[e];
-  const bool served = w.row >= 0 && first != ~0u;
-  if (blockIdx.y == 0 && threadIdx.x == 0 && status) status[e] = served;
+  const bool served = w.row >= 0 && w.first != ~0u;
+  if (y == 0 && tid == 0 && status) status[e] = served;
   if (!served) return;
-  const uint32_t have = v.pages_of(w.old), want = v.pages_of(w.length);
   const bool copied = w.shared >= 0;
-  if (blockIdx.y == 0) {
+  if (y == 0) {
+    const uint32_t have = v.pages_of(w.old), want = v.pages_of(w.length);
     int32_t* row = v.row(w.row);
-    for (uint32_t j = have + threadIdx.x; j < want; j += kCopyThreads) {
-      const int32_t page = free_list[first + copied + j - have];
+    for (uint32_t j = have + tid; j < want; j += kCopyThreads) {
+      const int32_t page = free_list[w.first + copied + j - have];
       row[j] = page;
       v.refs[page] = 1;
     }
-    for (uint32_t j = want + threadIdx.x; j < have; j += kCopyThreads) {
+    for (uint32_t j = want + tid; j < have; j += kCopyThreads) {
       const int32_t page = row[j];
       if (static_cast<uint32_t>(page) < v.num_pages) atomicSub(&v.refs[page], 1);
     }
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
       v.lengths[w.row] = w.length;
       if (copied) {
-        row[have - 1] = free_list[first];
-        v.refs[free_list[first]] = 1;
+        row[have - 1] = free_list[w.first];
+        v.refs[free_list[w.first]] = 1;
         atomicSub(&v.refs[w.shared], 1);
       }
     }
   }
   if (copied)
-    for (uint32_t c = blockIdx.y; c < planes.chunks; c += gridDim.y)
-      copy_chunk<kBytes>(planes, c, w.shared, free_list[first]);
+    for (uint32_t c = y; c < planes.chunks; c += chunks_at_once)
+      copy_chunk<kBytes>(planes, c, w.shared, free_list[w.first], tid);
+}
+
+// What entry e wants; passed over where another entry of its row comes later.
+__device__ __forceinline__ Want wanted(const PoolView& v, int32_t row, int32_t length,
+                                       uint32_t* need) {
+  Want w{-1, 0, length, -1, 0};
+  *need = 0;
+  if (static_cast<uint32_t>(row) >= v.num_rows || length < 0 ||
+      static_cast<uint64_t>(length) > static_cast<uint64_t>(v.max_pages) * v.page_tokens)
+    return w;
+  w.row = row;
+  w.old = max(0, v.lengths[row]);
+  const uint32_t have = v.pages_of(w.old), want = v.pages_of(length);
+  if (length > w.old && w.old % v.page_tokens != 0) {
+    const int32_t last = v.row(row)[have - 1];
+    if (static_cast<uint32_t>(last) < v.num_pages && v.refs[last] > 1) w.shared = last;
+  }
+  *need = (want > have ? want - have : 0) + (w.shared >= 0);
+  return w;
+}
+
+// owners: kPlanBlocks arrays of num_rows in global memory, null where one fits
+// shared memory. chunks_at_once: 0 leaves the changes to resize_apply_kernel.
+// A list that fits the threads of a block, on a pool of one strip, is planned
+// by the first block alone.
+template <int kBytes>
+__global__ void __launch_bounds__(kStripThreads)
+    resize_plan_kernel(const __grid_constant__ PlaneSet planes, PoolView v, uint32_t n,
+                       const int32_t* rows, const int32_t* lengths, uint32_t strips,
+                       int32_t* owners, Want* wants, uint32_t* needs, int32_t* free_list,
+                       bool* status, uint32_t chunks_at_once) {
+  extern __shared__ int32_t owner_smem[];
+  __shared__ uint32_t shared[2];
+  const uint32_t rank = cluster_rank();
+  const bool alone = strips == 1 && n <= kStripThreads;
+  int32_t* owner = owners ? owners + static_cast<uint64_t>(rank) * v.num_rows : owner_smem;
+  after_previous();
+  if (!alone || rank == 0) {
+    for (uint32_t r = threadIdx.x; r < v.num_rows; r += kStripThreads) owner[r] = -1;
+    uint32_t s0 = 0, s1 = 1, e0 = 0, e1 = n, page = 0;
+    if (!alone) {
+      plan_share(strips, rank, &s0, &s1);
+      plan_share(n, rank, &e0, &e1);
+    }
+    // free pages of this block's strips
+    uint32_t bits = 0, free_here = 0, need_here = 0, need = 0;
+    for (uint32_t s = s0; s < s1; s++) {
+      bits = free_bits(strip_counts(v, s, &page));
+      free_here += __popc(bits);
+    }
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < n; e += kStripThreads) {
+      const int32_t r = rows[e];
+      if (static_cast<uint32_t>(r) < v.num_rows) atomicMax(&owner[r], static_cast<int32_t>(e));
+    }
+    // this block's entries
+    Want w;
+    bool mine = false;  // w is that of the thread's one entry
+    const bool single = e1 - e0 <= kStripThreads;
+    if (single && e0 + threadIdx.x < e1) {
+      w = wanted(v, rows[e0 + threadIdx.x], lengths[e0 + threadIdx.x], &need);
+      mine = true;
+    }
+    __syncthreads();
+    if (mine && w.row >= 0 &&
+        atomicMax(&owner[w.row], -1) != static_cast<int32_t>(e0 + threadIdx.x)) {  // a read
+      w.row = -1;
+      need = 0;
+    }
+    need_here = need;
+    for (uint32_t e = e0 + threadIdx.x; !single && e < e1; e += kStripThreads) {
+      w = wanted(v, rows[e], lengths[e], &need);
+      if (w.row >= 0 && atomicMax(&owner[w.row], -1) != static_cast<int32_t>(e)) {
+        w.row = -1;
+        need = 0;
+      }
+      wants[e] = w;
+      needs[e] = need;
+      need_here += need;
+    }
+    uint32_t at, first, free_all, need_all, free_before = 0, need_before = 0, total;
+    block_exclusive2(free_here, need_here, &at, &first, &free_all, &need_all);
+    if (!alone)
+      exchange(free_all, need_all, rank, shared, &free_before, &free_all, &need_before, &need_all);
+    // places in the list, in the entries' order. Served: needs nothing, or all
+    // that is wanted up to here is there (the sum stays below 2^32: rows
+    // differ, and each wants max_pages + 1 at most).
+    if (mine) {
+      first += need_before;
+      w.first = need == 0 || first + need <= free_all ? first : ~0u;
+      wants[e0 + threadIdx.x] = w;
+    }
+    for (uint32_t e = e0; !single && e < e1; e += kStripThreads) {
+      const bool on = e + threadIdx.x < e1;
+      need = on ? needs[e + threadIdx.x] : 0;
+      first = need_before + block_exclusive(need, &total);
+      if (on) wants[e + threadIdx.x].first = need == 0 || first + need <= free_all ? first : ~0u;
+      need_before += total;
+    }
+    if (s1 - s0 == 1 && free_before < need_all) {
+      at += free_before;
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (bits >> k & 1) free_list[at++] = page + k;
+    }
+    for (uint32_t s = s0; s1 - s0 > 1 && s < s1 && free_before < need_all; s++) {
+      bits = free_bits(strip_counts(v, s, &page));
+      at = free_before + block_exclusive(__popc(bits), &total);
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (bits >> k & 1) free_list[at++] = page + k;
+      free_before += total;
+    }
+  }
+  cluster_sync();
+  const uint32_t team = (rank * kStripThreads + threadIdx.x) / kCopyThreads;
+  constexpr uint32_t kTeams = kPlanBlocks * kStripThreads / kCopyThreads;
+  for (uint32_t u = team; u < n * chunks_at_once; u += kTeams)
+    resize_entry<kBytes>(planes, v, wants, free_list, status, u / chunks_at_once,
+                         u % chunks_at_once, chunks_at_once, threadIdx.x % kCopyThreads);
+}
+
+template <int kBytes>
+__global__ void __launch_bounds__(kCopyThreads)
+    resize_apply_kernel(const __grid_constant__ PlaneSet planes, PoolView v, const Want* wants,
+                        const int32_t* free_list, bool* status) {
+  after_previous();
+  resize_entry<kBytes>(planes, v, wants, free_list, status, blockIdx.x, blockIdx.y, gridDim.y,
+                       threadIdx.x);
 }
 
 // ---- compact ----------------------------------------------------------------
 // L pages in use. The rank of a page in use is the number of those before it.
 // Pages in use below L stay. The i-th hole (free page below L) gets the i-th
 // page in use behind, whose rank is A + i, where A pages in use lie below L.
-// Three launches: live pages per strip; the lists of holes and of movers by
-// rank, and the map (a mover's entry holds -2 - rank until its new number is
-// written, and both mean the same to a reader); the moves, the table and the
-// counts.
-
-__global__ void __launch_bounds__(kStripThreads)
-    compact_count_kernel(PoolView v, uint32_t* counts) {
-  after_previous();
-  uint32_t first, total;
-  const int4 c = strip_counts(v, blockIdx.x, &first);
-  block_exclusive(__popc(live_bits(c)), &total);
-  if (threadIdx.x == 0) counts[blockIdx.x] = total;
-}
+// The plan: the lists of holes and of movers by rank, and the map (a mover's
+// entry holds -2 - rank until its new number is written, and both mean the same
+// to a reader). Then the moves, the table and the counts, in the same launch in
+// a small pool, else in a second one.
 
 struct Compact {
   uint32_t live;   // L
   uint32_t below;  // A
 };
 
-__global__ void __launch_bounds__(kStripThreads)
-    compact_list_kernel(PoolView v, uint32_t strips, const uint32_t* counts, int32_t* page_map,
-                        int32_t* holes, int32_t* movers, int32_t* refs_out, Compact* result) {
-  after_previous();
-  uint32_t before, live, ignored, first;
-  strip_base(counts, blockIdx.x, strips, &before, &live);
-  const int4 c = strip_counts(v, blockIdx.x, &first);
-  const uint32_t bits = live_bits(c);
-  uint32_t rank = before + block_exclusive(__popc(bits), &ignored);
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    result->live = live;
-    if (live == v.num_pages) result->below = live;
-  }
-  const int32_t count[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const uint32_t page = first + k;
-    if (page >= v.num_pages) break;
-    const bool used = bits >> k & 1;
-    if (page == live) result->below = rank;
-    int32_t to = -1;
-    if (page < live) {
-      if (used)
-        to = page;
-      else
-        holes[page - rank] = page;
-      if (used && refs_out != v.refs) refs_out[page] = count[k];
-    } else if (used) {
-      movers[rank] = page;
-      to = -2 - static_cast<int32_t>(rank);
-    } else if (refs_out != v.refs) {
-      refs_out[page] = 0;
-    }
-    page_map[page] = to;
-    rank += used;
-  }
-}
+constexpr uint32_t kTableChunk = 1024;  // table entries of a team's step
 
-constexpr uint32_t kTableChunk = 1024;  // table entries of a block's step
+struct Moves {
+  int32_t* page_map;
+  int32_t* holes;
+  int32_t* movers;
+  int32_t* refs_out;
+  int32_t* table_out;
+  Compact* result;
+};
 
+// The share of team `team` of `teams`, each kCopyThreads threads.
 template <int kBytes>
-__global__ void __launch_bounds__(kCopyThreads)
-    compact_move_kernel(const __grid_constant__ PlaneSet planes, PoolView v, int32_t* page_map,
-                        const int32_t* holes, const int32_t* movers, const int32_t* refs,
-                        int32_t* refs_out, int32_t* table_out, const Compact* result) {
-  after_previous();
-  const uint32_t live = result->live, below = result->below, moved = live - below;
+__device__ __forceinline__ void compact_move(const PlaneSet& planes, const PoolView& v,
+                                             const Moves& m, uint32_t team, uint32_t teams,
+                                             uint32_t tid) {
+  const uint32_t below = m.result->below, moved = m.result->live - below;
   const uint32_t row_chunks = (v.max_pages + kTableChunk - 1) / kTableChunk;
   const uint64_t table_units = static_cast<uint64_t>(v.num_rows) * row_chunks;
   const uint64_t pair_units = (moved + kCopyThreads - 1) / kCopyThreads;
   const uint64_t copy_units = static_cast<uint64_t>(moved) * planes.chunks;
-  for (uint64_t u = blockIdx.x; u < copy_units + pair_units + table_units; u += gridDim.x) {
+  for (uint64_t u = team; u < copy_units + pair_units + table_units; u += teams) {
     if (u < copy_units) {
       const uint32_t i = static_cast<uint32_t>(u / planes.chunks);
-      copy_chunk<kBytes>(planes, static_cast<uint32_t>(u - static_cast<uint64_t>(i) * planes.chunks),
-                         movers[below + i], holes[i]);
+      copy_chunk<kBytes>(planes,
+                         static_cast<uint32_t>(u - static_cast<uint64_t>(i) * planes.chunks),
+                         m.movers[below + i], m.holes[i], tid);
     } else if (u < copy_units + pair_units) {
-      const uint32_t i = static_cast<uint32_t>(u - copy_units) * kCopyThreads + threadIdx.x;
+      const uint32_t i = static_cast<uint32_t>(u - copy_units) * kCopyThreads + tid;
       if (i < moved) {
-        const int32_t from = movers[below + i], to = holes[i];
-        refs_out[to] = refs[from];
-        refs_out[from] = 0;
-        __stcg(page_map + from, to);
+        const int32_t from = m.movers[below + i], to = m.holes[i];
+        m.refs_out[to] = v.refs[from];
+        m.refs_out[from] = 0;
+        __stcg(m.page_map + from, to);
       }
     } else {
       const uint64_t k = u - copy_units - pair_units;
       const uint32_t r = static_cast<uint32_t>(k / row_chunks);
-      const uint32_t j0 = static_cast<uint32_t>(k - static_cast<uint64_t>(r) * row_chunks) * kTableChunk;
-      const uint32_t pages = v.pages_of(v.lengths[r]);
-      const uint32_t last = min(pages, j0 + kTableChunk);
-      for (uint32_t j = j0 + threadIdx.x; j < last; j += kCopyThreads) {
+      const uint32_t j0 =
+          static_cast<uint32_t>(k - static_cast<uint64_t>(r) * row_chunks) * kTableChunk;
+      const uint32_t last = min(v.pages_of(v.lengths[r]), j0 + kTableChunk);
+      for (uint32_t j = j0 + tid; j < last; j += kCopyThreads) {
         const uint32_t page = static_cast<uint32_t>(v.row(r)[j]);
         int32_t to = -1;
-        if (page < v.num_pages) to = __ldcg(page_map + page);
-        if (to < -1) to = holes[-2 - to - static_cast<int32_t>(below)];
-        table_out[r * v.stride + j] = to;
+        if (page < v.num_pages) to = __ldcg(m.page_map + page);
+        if (to < -1) to = m.holes[-2 - to - static_cast<int32_t>(below)];
+        m.table_out[r * v.stride + j] = to;
       }
     }
   }
+}
+
+template <int kBytes>
+__global__ void __launch_bounds__(kStripThreads)
+    compact_plan_kernel(const __grid_constant__ PlaneSet planes, PoolView v, uint32_t strips,
+                        Moves m, bool move) {
+  __shared__ uint32_t shared[2];
+  const uint32_t block = cluster_rank();
+  after_previous();
+  uint32_t s0, s1, live_here = 0, first, total, at, before = 0, live, none, nil;
+  plan_share(strips, block, &s0, &s1);
+  int4 c;
+  for (uint32_t s = s0; s < s1; s++) {
+    c = strip_counts(v, s, &first);
+    live_here += __popc(live_bits(c));
+  }
+  at = block_exclusive(live_here, &live);
+  if (strips > 1) exchange(live, 0, block, shared, &before, &live, &none, &nil);
+  if (s0 == 0 && s1 > 0 && threadIdx.x == 0) {
+    m.result->live = live;
+    if (live == v.num_pages) m.result->below = live;
+  }
+  for (uint32_t s = s0; s < s1; s++) {
+    if (s1 - s0 > 1) {
+      c = strip_counts(v, s, &first);
+      at = block_exclusive(__popc(live_bits(c)), &total);
+    }
+    const uint32_t bits = live_bits(c);
+    uint32_t rank = before + at;
+    if (s1 - s0 > 1) before += total;
+    const int32_t count[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const uint32_t page = first + k;
+      if (page >= v.num_pages) break;
+      const bool used = bits >> k & 1;
+      if (page == live) m.result->below = rank;
+      int32_t to = -1;
+      if (page < live) {
+        if (used)
+          to = page;
+        else
+          m.holes[page - rank] = page;
+        if (used && m.refs_out != v.refs) m.refs_out[page] = count[k];
+      } else if (used) {
+        m.movers[rank] = page;
+        to = -2 - static_cast<int32_t>(rank);
+      } else if (m.refs_out != v.refs) {
+        m.refs_out[page] = 0;
+      }
+      m.page_map[page] = to;
+      rank += used;
+    }
+  }
+  cluster_sync();
+  if (move)
+    compact_move<kBytes>(planes, v, m, (block * kStripThreads + threadIdx.x) / kCopyThreads,
+                         kPlanBlocks * kStripThreads / kCopyThreads, threadIdx.x % kCopyThreads);
+}
+
+template <int kBytes>
+__global__ void __launch_bounds__(kCopyThreads)
+    compact_move_kernel(const __grid_constant__ PlaneSet planes, PoolView v, Moves m) {
+  after_previous();
+  compact_move<kBytes>(planes, v, m, blockIdx.x, gridDim.x, threadIdx.x);
 }
 
 // The pool's device while in scope.
@@ -459,6 +635,14 @@ class OnDevice {
 }  // namespace
 
 class PagesImpl {
+  static constexpr int kMostShared = 200 * 1024;
+  static constexpr uint32_t kOneLaunchChunks = 256, kOneLaunchMoves = 1024;
+  static constexpr size_t kOneLaunchEntries = 1 << 15;
+  // Blocks of a move per SM: 8 stay resident and take 12 units each one after
+  // the other (90 us for 472 MB), 32 hide a unit's chain of loads behind the
+  // next block's (81), 256 mostly find nothing left to do (99).
+  static constexpr uint32_t kMoveBlocks = 32;
+
  public:
   PagesImpl(const hkv_pages_options& o, const hkv_allocator* allocator) : mem_(allocator) {
     HKV_REQUIRE(o.num_pages > 0 && o.page_tokens > 0 && o.num_rows > 0 && o.max_pages > 0,
@@ -503,7 +687,7 @@ class PagesImpl {
     }
     planes_.chunks = static_cast<uint32_t>(chunks);
     view_ = PoolView{o.refs, o.table, o.lengths, o.table_stride ? o.table_stride : o.max_pages,
-                     o.num_pages, o.page_tokens, o.num_rows, o.max_pages};
+                      o.num_pages, o.page_tokens, o.num_rows, o.max_pages};
     if (o.device_id >= 0)
       device_ = o.device_id;
     else
@@ -518,15 +702,21 @@ class PagesImpl {
       bytes += (b + 255) / 256 * 256;
       return at;
     };
-    const size_t a_counts = part(strips_ * 4ull), a_result = part(sizeof(Compact));
+    const size_t a_arrived = part(4), a_result = part(sizeof(Compact));
     const size_t a_list = part(o.num_pages * 4ull), a_movers = part(o.num_pages * 4ull);
     const size_t a_map = part(o.num_pages * 4ull);
     const size_t a_forks = part(o.num_rows * sizeof(Fork));
     const size_t a_wants = part(o.num_rows * sizeof(Want));
-    const size_t a_needs = part(o.num_rows * 4ull), a_first = part(o.num_rows * 4ull);
-    const size_t a_staged = part(static_cast<size_t>(o.num_rows) * o.max_pages * 4);
+    const size_t a_needs = part(o.num_rows * 4ull);
+    const bool many_rows = o.num_rows * 4ull > kMostShared;
+    const size_t a_owners = part(many_rows ? o.num_rows * 4ull * kPlanBlocks : 0);
+    // entries of forked rows, for lists that take two launches
+    const bool stages = fork_smem(o.num_rows, o.num_rows) > kMostShared ||
+                        static_cast<size_t>(o.num_rows) * o.max_pages > kOneLaunchEntries;
+    const size_t a_staged =
+        part(stages ? static_cast<size_t>(o.num_rows) * o.max_pages * 4 : 0);
     scratch_ = static_cast<uint8_t*>(mem_.device(bytes));
-    counts_ = reinterpret_cast<uint32_t*>(scratch_ + a_counts);
+    arrived_ = reinterpret_cast<uint32_t*>(scratch_ + a_arrived);
     result_ = reinterpret_cast<Compact*>(scratch_ + a_result);
     list_ = reinterpret_cast<int32_t*>(scratch_ + a_list);
     movers_ = reinterpret_cast<int32_t*>(scratch_ + a_movers);
@@ -534,8 +724,21 @@ class PagesImpl {
     forks_ = reinterpret_cast<Fork*>(scratch_ + a_forks);
     wants_ = reinterpret_cast<Want*>(scratch_ + a_wants);
     needs_ = reinterpret_cast<uint32_t*>(scratch_ + a_needs);
-    first_ = reinterpret_cast<uint32_t*>(scratch_ + a_first);
+    if (many_rows) owners_ = reinterpret_cast<int32_t*>(scratch_ + a_owners);
     staged_ = reinterpret_cast<int32_t*>(scratch_ + a_staged);
+    try {
+      CUDA_TRY(cudaMemset(arrived_, 0, 4));
+      CUDA_TRY(cudaDeviceSynchronize());
+      CUDA_TRY(cudaFuncSetAttribute(fork_columns_kernel,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+      with_width([&](auto width) {
+        CUDA_TRY(cudaFuncSetAttribute(resize_plan_kernel<decltype(width)::value>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+      });
+    } catch (...) {
+      mem_.free_device(scratch_);
+      throw;
+    }
   }
 
   ~PagesImpl() {
@@ -568,6 +771,12 @@ class PagesImpl {
     check_list(src, "src");
     check_list(dst, "dst");
     OnDevice on(device_);
+    const size_t smem = fork_smem(view_.num_rows, n);
+    if (n * view_.max_pages <= kOneLaunchEntries && smem <= kMostShared) {
+      launch(fork_columns_kernel, (view_.max_pages + kForkColumns - 1) / kForkColumns,
+             kForkColumnThreads, smem, s, 1, view_, static_cast<uint32_t>(n), src, dst, arrived_);
+      return;
+    }
     const dim3 grid(static_cast<uint32_t>(n), (view_.max_pages + kForkChunk - 1) / kForkChunk);
     launch(fork_read_kernel, grid, kForkThreads, 0, s, 1, view_, static_cast<uint32_t>(n), src, dst,
            forks_, staged_);
@@ -582,17 +791,21 @@ class PagesImpl {
     check_list(lengths, "lengths");
     OnDevice on(device_);
     const uint32_t m = static_cast<uint32_t>(n);
-    launch(resize_count_kernel, strips_ + (m + kStripWarps - 1) / kStripWarps, kStripThreads, 0, s,
-           1, view_, m, rows, lengths, strips_, counts_, wants_, needs_);
-    launch(resize_list_kernel, strips_ + 1, kStripThreads, 0, s, 1, view_, m, strips_, counts_,
-           needs_, first_, list_);
-    // blocks of an entry: as many as its page copy can use, few where there
-    // are entries enough to fill the device
-    const uint32_t fill = std::max(1u, static_cast<uint32_t>(sm_count_) * 16 / m);
-    const dim3 grid(m, std::max(1u, std::min(planes_.chunks, fill)));
+    // in one launch up to some copied chunks per team of threads
+    const uint32_t chunks = std::max(1u, planes_.chunks);
+    const bool one = static_cast<uint64_t>(m) * chunks <= kOneLaunchChunks;
+    const uint32_t at_once = one ? chunks : 0;
+    const size_t smem = owners_ ? 0 : view_.num_rows * 4ull;
     with_width([&](auto width) {
-      launch(resize_apply_kernel<decltype(width)::value>, grid, kCopyThreads, 0, s, 1, planes_,
-             view_, wants_, first_, list_, status);
+      constexpr int kBytes = decltype(width)::value;
+      launch(resize_plan_kernel<kBytes>, kPlanBlocks, kStripThreads, smem, s, kPlanBlocks, planes_,
+             view_, m, rows, lengths, strips_, owners_, wants_, needs_, list_, status, at_once);
+      if (one) return;
+      // blocks of an entry: as many as its page copy can use, few where there
+      // are entries enough to fill the device
+      const uint32_t fill = std::max(1u, static_cast<uint32_t>(sm_count_) * 16 / m);
+      launch(resize_apply_kernel<kBytes>, dim3(m, std::min(chunks, fill)),
+             kCopyThreads, 0, s, 1, planes_, view_, wants_, list_, status);
     });
   }
 
@@ -618,18 +831,20 @@ class PagesImpl {
     if (table_out) check_list(table_out, "table_out"); else table_out = view_.table;
     if (refs_out) check_list(refs_out, "refs_out"); else refs_out = view_.refs;
     OnDevice on(device_);
-    launch(compact_count_kernel, strips_, kStripThreads, 0, s, 1, view_, counts_);
-    launch(compact_list_kernel, strips_, kStripThreads, 0, s, 1, view_, strips_, counts_, page_map,
-           list_, movers_, refs_out, result_);
+    const Moves m{page_map, list_, movers_, refs_out, table_out, result_};
     // at most half of the pages can move
     const uint64_t units = (view_.num_pages / 2 + 1ull) * (planes_.chunks + 1ull) +
                            static_cast<uint64_t>(view_.num_rows) *
                                ((view_.max_pages + kTableChunk - 1) / kTableChunk);
-    const uint32_t grid =
-        static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(sm_count_) * 8, units));
+    const bool one = units <= kOneLaunchMoves;
     with_width([&](auto width) {
-      launch(compact_move_kernel<decltype(width)::value>, grid, kCopyThreads, 0, s, 1, planes_,
-             view_, page_map, list_, movers_, view_.refs, refs_out, table_out, result_);
+      constexpr int kBytes = decltype(width)::value;
+      launch(compact_plan_kernel<kBytes>, kPlanBlocks, kStripThreads, 0, s, kPlanBlocks, planes_,
+             view_, strips_, m, one);
+      if (one) return;
+      launch(compact_move_kernel<kBytes>,
+             static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(sm_count_) * kMoveBlocks, units)),
+             kCopyThreads, 0, s, 1, planes_, view_, m);
     });
   }
 
@@ -657,12 +872,13 @@ class PagesImpl {
   uint32_t strips_ = 0;
   int device_ = 0, sm_count_ = 148;
   uint8_t* scratch_ = nullptr;
-  uint32_t* counts_ = nullptr;  // per strip
+  uint32_t* arrived_ = nullptr;  // blocks of a fork that have read the lengths
   Compact* result_ = nullptr;
   int32_t *list_ = nullptr, *movers_ = nullptr, *map_ = nullptr;  // per page
   Fork* forks_ = nullptr;  // per list entry
   Want* wants_ = nullptr;
-  uint32_t *needs_ = nullptr, *first_ = nullptr;
+  uint32_t* needs_ = nullptr;
+  int32_t* owners_ = nullptr;  // per row, for each block of a plan
   int32_t* staged_ = nullptr;  // entries of forked rows
 };
 

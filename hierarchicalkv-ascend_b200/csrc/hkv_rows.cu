@@ -111,23 +111,6 @@ __device__ __forceinline__ uint32_t scan_over_warps(uint16_t* cnt, uint32_t warp
   return before;
 }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n"
-               "barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// word `p` of this block's shared memory, in block `rank` of the cluster
-__device__ __forceinline__ uint32_t load_remote(const uint32_t* p, uint32_t rank) {
-  uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(p)), r, v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(r) : "memory");
-  return v;
-}
-
 // One launch: `blocks` blocks of one cluster, block b takes the places from
 // b * blockDim.x * kItems. The rows of order are written from shared memory
 // in the block's sorted order, so that a group's run is written in whole
@@ -179,8 +162,8 @@ __global__ void __launch_bounds__(kClusterThreads)
     sum += all;
     own += mine_all[g];
   }
-  uint32_t run = block_exclusive(sum, &kept);
-  uint32_t run_here = block_exclusive(own, &here);
+  uint32_t run, run_here;
+  block_exclusive2(sum, own, &run, &run_here, &kept, &here);
   for (uint32_t g = g0; g < g1; g++) {
     if (me == 0) offsets[g] = run;
     start[g] += run;

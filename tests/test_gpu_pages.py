@@ -41,8 +41,8 @@ class Model:
 
     def entries(self, rows):
         """List entries that count: rows that exist, the last of each."""
-        return [k for k, r in enumerate(rows)
-                if 0 <= r < len(self.lengths) and r not in rows[k + 1:]]
+        last = {r: k for k, r in enumerate(rows)}
+        return [k for k, r in enumerate(rows) if 0 <= r < len(self.lengths) and last[r] == k]
 
     def fork(self, src, dst):
         rows = [list(r) for r in self.table]
@@ -60,7 +60,7 @@ class Model:
     def resize(self, rows, lengths):
         refs = list(self.refs)
         free = [p for p, c in enumerate(refs) if c == 0]
-        counts, status, wanted = self.entries(rows), [], 0
+        counts, status, wanted = set(self.entries(rows)), [], 0
         for k, (r, n) in enumerate(zip(rows, lengths)):
             if k not in counts or n < 0 or n > self.width * self.size:
                 status.append(False)
@@ -306,6 +306,22 @@ def test_any_order_of_calls(seed, pages, size, rows, width, plane_bytes):
         else:
             b.compact(beside=bool(rng.integers(0, 2)))
     assert all(c >= 0 for c in b.pool.refs.tolist())
+
+
+@pytest.mark.parametrize("rows", [4000, 6000, 60000])
+def test_many_rows(rows):
+    """Lists and pools of the size where the calls take their scratch elsewhere."""
+    rng = np.random.default_rng(rows)
+    b = Both(40000, 4, rows, 3, (16,), rows)
+    some = rng.permutation(rows)[:rows // 2].tolist()
+    b.resize(some, rng.integers(0, 9, len(some)).tolist())
+    every = rng.integers(-1, rows + 1, rows).tolist()
+    b.fork(every, rng.permutation(rows).tolist())
+    b.resize(every, rng.integers(-1, 14, rows).tolist())
+    b.fork(rng.permutation(rows).tolist(), every)
+    b.free(some)
+    b.compact()
+    b.fork([1, 2], [2, 1])
 
 
 def test_wide_table_rows_and_given_state():
