@@ -34,7 +34,11 @@ void launch(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem,
   a[1].val.clusterDim.y = a[1].val.clusterDim.z = 1;
   c.attrs = a;
   c.numAttrs = cluster > 1 ? 2 : 1;
-  CUDA_TRY(cudaLaunchKernelEx(&c, kernel, std::forward<Args>(args)...));
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, std::forward<Args>(args)...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // not left for the next call to find
+    throw HkvError{HKV_ERR_CUDA, std::string("kernel launch: ") + cudaGetErrorString(e)};
+  }
 }
 
 __device__ __forceinline__ void after_previous() {

@@ -278,7 +278,7 @@ def test_table_entries_out_of_range_are_passed_over():
 
 @pytest.mark.parametrize("seed,pages,size,rows,width,plane_bytes", [
     (1, 40, 4, 7, 9, (32, 5)), (2, 4100, 16, 60, 40, (16,)), (3, 9000, 8, 300, 64, (16, 16)),
-    (4, 5, 1, 3, 5, (48,)), (5, 130, 64, 33, 4, ()), (6, 3000, 3, 9, 1500, (20,))])
+    (4, 5, 1, 3, 5, (48,)), (5, 130, 64, 33, 4, ()), (6, 3000, 3, 9, 1500, (20,)), (7, 3000, 3, 40, 1500, (20,))])
 def test_any_order_of_calls(seed, pages, size, rows, width, plane_bytes):
     rng = np.random.default_rng(seed)
     b = Both(pages, size, rows, width, plane_bytes, seed)
@@ -322,6 +322,38 @@ def test_many_rows(rows):
     b.free(some)
     b.compact()
     b.fork([1, 2], [2, 1])
+
+
+def test_pages_of_several_chunks_and_many_entries():
+    """Page copies that a few blocks of an entry take in steps."""
+    b = Both(2700, 4, 1300, 2, (33000, 16), 4)
+    first = list(range(0, 1300, 2))
+    b.resize(first, [6] * 650)
+    b.fork(first, [r + 1 for r in first])
+    b.resize([r + 1 for r in first], [7] * 650)
+    b.compact()
+
+
+def test_two_pools_on_two_streams():
+    """Pools share nothing: their calls may overlap."""
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    pools = [Both(5000, 4, 200, 12, (4096,), k) for k in range(2)]
+    lists = [i32(list(range(200))), i32([30] * 200), i32(list(range(100, 200)) + list(range(100)))]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for b, s in zip(pools, streams):
+            b.pool.resize(200, lists[0], lists[1], stream=s)
+            b.pool.fork(200, lists[0], lists[2], stream=s)
+            b.pool.compact(stream=s)
+            b.pool.free(100, lists[2], stream=s)
+    torch.cuda.synchronize()
+    for b in pools:
+        for _ in range(3):
+            b.model.resize(lists[0].tolist(), lists[1].tolist())
+            b.model.fork(lists[0].tolist(), lists[2].tolist())
+            b.model.compact()
+            b.model.free(lists[2].tolist()[:100])
+        b.check()
 
 
 def test_wide_table_rows_and_given_state():

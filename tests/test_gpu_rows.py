@@ -126,6 +126,22 @@ def test_group_tokens_on_other_streams():
     assert np.array_equal(order.cpu().numpy(), want[2])
 
 
+def test_group_tokens_on_two_streams_at_once():
+    n, groups = 300000, 100
+    ids = [torch.randint(0, groups, (n,), generator=seeded(k), device="cuda") for k in range(2)]
+    out = [(i32(groups + 1), i32(n), i32(n)) for _ in ids]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for k, s in enumerate(streams):  # each call its own scratch, from its stream's pool
+            H.group_tokens(n, ids[k], groups, *out[k], stream=s)
+    torch.cuda.synchronize()
+    for k in range(2):
+        want = sorted_reference(ids[k], groups)
+        assert np.array_equal(out[k][1].cpu().numpy(), want[1])
+        assert np.array_equal(out[k][2].cpu().numpy(), want[2])
+
+
 # ---- dispatch_rows -----------------------------------------------------------
 
 
