@@ -841,24 +841,40 @@ def _list(t, name, n, dtype):
     raise HkvException(f"{name} must be contiguous")
 
 
-def _one_device(tensors):
-    """Index of the CUDA device that all the tensors are on."""
+def _one_device(*tensors):
+    """Index of the CUDA device that all the tensors (or None) are on."""
     index = tensors[0].get_device()
-    _refuse_unless(index >= 0, "the tensors must be on a CUDA device")
+    if index < 0:
+        raise HkvException("the tensors must be on a CUDA device")
     for t in tensors:
-        _refuse_unless(t.get_device() == index, "the tensors are on different devices")
+        if t is not None and t.get_device() != index:
+            raise HkvException("the tensors are on different devices")
     return index
 
 
 def _call_on(index, stream, fn, *args):
     """fn(*args, stream) with device `index` current."""
-    t = _torch()
+    t = _TORCH
     stream = t.stream(index) if stream is None else _stream(stream)
     if t.device() == index:
-        _check(fn(*args, stream))
+        status = fn(*args, stream)
     else:
         with t.torch.cuda.device(index):
-            _check(fn(*args, stream))
+            status = fn(*args, stream)
+    if status:
+        _check(status)
+
+
+def _row_kind(dtype):
+    kind = _torch().rows.get(dtype)
+    if kind is None:
+        raise HkvException(f"rows of {dtype} are not supported")
+    return kind
+
+
+def _not_negative(n):
+    if n < 0:
+        raise HkvException("n must not be negative")
 
 
 def group_workspace(n: int, num_groups: int) -> int:
@@ -880,31 +896,27 @@ def group_tokens(n, groups, num_groups, offsets, positions, order=None, workspac
     uint8 tensor of group_workspace(n, num_groups) bytes, allocated here when
     None; calls that may overlap need their own."""
     torch = _torch()
-    _refuse_unless(n >= 0, "n must not be negative")
+    _not_negative(n)
     ids = torch.ids.get(groups.dtype)
     if ids is None:
         raise HkvException(f"groups must be int32 or int64, not {groups.dtype}")
     g = _list(groups, "groups", n, groups.dtype)
     p = _list(positions, "positions", n, torch.int32)
     f = _list(offsets, "offsets", num_groups + 1, torch.int32)
-    tensors = [groups, positions, offsets]
-    r = None
-    if order is not None:
-        r = _list(order, "order", n, torch.int32)
-        tensors.append(order)
-    size = group_workspace(n, num_groups) if workspace is None else 0
-    if workspace is not None:
-        size = workspace.nbytes
-        _refuse_unless(workspace.is_contiguous(), "workspace must be contiguous")
-        tensors.append(workspace)
-    index = _one_device(tensors)
+    r = None if order is None else _list(order, "order", n, torch.int32)
+    index = _one_device(groups, positions, offsets, order, workspace)
     if workspace is None:
+        size = group_workspace(n, num_groups)
         cuda = torch.torch.cuda
         if isinstance(stream, int):
             stream = cuda.ExternalStream(stream, index)
         # from the pool of the stream that uses it
         with cuda.stream(stream or cuda.current_stream(index)):
             workspace = torch.torch.empty(size, dtype=torch.torch.uint8, device=groups.device)
+    else:
+        size = workspace.nbytes
+        if not workspace.is_contiguous():
+            raise HkvException("workspace must be contiguous")
     _call_on(index, stream, lib().hkv_group_tokens, n, g, ids, num_groups, f, p, r,
              workspace.data_ptr(), size)
 
@@ -912,10 +924,11 @@ def group_tokens(n, groups, num_groups, offsets, positions, order=None, workspac
 def _positions(n, positions):
     """(address, slots) of the int32 positions [tokens, slots]."""
     shape = positions.shape
-    _refuse_unless(len(shape) == 2 and shape[1] > 0, "positions must be [tokens, slots]")
+    if len(shape) != 2 or shape[1] == 0:
+        raise HkvException("positions must be [tokens, slots]")
     if n > shape[0]:
         raise HkvException(f"positions has {shape[0]} tokens, fewer than {n}")
-    return _list(positions, "positions", 0, _torch().int32), shape[1]
+    return _list(positions, "positions", 0, _TORCH.int32), shape[1]
 
 
 def dispatch_rows(n, x, positions, rows, stream=None):
@@ -923,21 +936,20 @@ def dispatch_rows(n, x, positions, rows, stream=None):
     x: [tokens, dim], positions: int32 [tokens, slots], rows: [rows, dim]; a
     position outside rows is passed over and rows that no place has stay as
     they were. The gradient: combine_rows(n, grad_rows, positions, None, grad_x)."""
-    _refuse_unless(n >= 0, "n must not be negative")
+    _not_negative(n)
     _, dim, x_stride = _matrix(x, "x", n)
     num_rows, width, rows_stride = _matrix(rows, "rows")
-    _refuse_unless(width == dim and rows.dtype == x.dtype, "x and rows differ in dim or type")
-    kind = _torch().rows.get(x.dtype)
-    if kind is None:
-        raise HkvException(f"rows of {x.dtype} are not supported")
+    kind = _row_kind(x.dtype)
+    if width != dim or rows.dtype is not x.dtype:
+        raise HkvException("x and rows differ in dim or type")
     p, slots = _positions(n, positions)
-    index = _one_device((x, positions, rows))
+    index = _one_device(x, positions, rows)
     _call_on(index, stream, lib().hkv_dispatch_rows, n, slots, dim, kind, x.data_ptr(),
              x_stride, p, num_rows, rows.data_ptr(), rows_stride)
 
 
 def _weights(weights, name, n, slots, kind):
-    shape, got = weights.shape, _torch().rows.get(weights.dtype)
+    shape, got = weights.shape, _TORCH.rows.get(weights.dtype)
     if (len(shape) == 2 and shape[1] == slots and shape[0] >= n and weights.is_contiguous()
             and (got == 0 or got == kind)):
         return got
@@ -964,27 +976,23 @@ def combine_rows(n, rows, positions, weights, out, stream=None, slots=None):
     out: [tokens, dim]. positions None: the row of place (t, s) is t * slots +
     s (what find wrote for the keys of n tokens), with slots as given or those
     of weights. Summed in float32, rounded once."""
-    _refuse_unless(n >= 0, "n must not be negative")
+    _not_negative(n)
     num_rows, dim, rows_stride = _matrix(rows, "rows")
     _, width, out_stride = _matrix(out, "out", n)
-    _refuse_unless(width == dim and rows.dtype == out.dtype, "rows and out differ in dim or type")
-    kind = _torch().rows.get(rows.dtype)
-    if kind is None:
-        raise HkvException(f"rows of {rows.dtype} are not supported")
-    tensors = [rows, out]
+    kind = _row_kind(rows.dtype)
+    if width != dim or out.dtype is not rows.dtype:
+        raise HkvException("rows and out differ in dim or type")
     if positions is not None:
         p, slots = _positions(n, positions)
-        tensors.append(positions)
     else:
         p, slots = None, _by_place(slots, weights)
-    w = w_kind = None
+    w, w_kind = None, 0
     if weights is not None:
         w_kind = _weights(weights, "weights", n, slots, kind)
         w = weights.data_ptr()
-        tensors.append(weights)
-    index = _one_device(tensors)
+    index = _one_device(rows, out, positions, weights)
     _call_on(index, stream, lib().hkv_combine_rows, n, slots, dim, kind, rows.data_ptr(),
-             rows_stride, num_rows, p, w, w_kind or 0, out.data_ptr(), out_stride)
+             rows_stride, num_rows, p, w, w_kind, out.data_ptr(), out_stride)
 
 
 def combine_rows_backward(n, rows, positions, weights, grad_out, grad_rows=None,
@@ -995,42 +1003,37 @@ def combine_rows_backward(n, rows, positions, weights, grad_out, grad_rows=None,
     without a row), either left out when None. Each row may be the row of one
     place only. rows may be None when grad_weights is. Without positions, slots
     as given or those of weights or grad_weights."""
-    _refuse_unless(n >= 0, "n must not be negative")
+    _not_negative(n)
     _, dim, out_stride = _matrix(grad_out, "grad_out", n)
-    kind = _torch().rows.get(grad_out.dtype)
-    if kind is None:
-        raise HkvException(f"rows of {grad_out.dtype} are not supported")
+    kind = _row_kind(grad_out.dtype)
     _refuse_unless(rows is not None or grad_weights is None, "grad_weights needs rows")
     if grad_rows is None and grad_weights is None:
         return
-    tensors, num_rows, rows_stride, grad_stride = [grad_out], None, 0, 0
+    num_rows, rows_stride, grad_stride = None, 0, 0
     for t, name in ((rows, "rows"), (grad_rows, "grad_rows")):
         if t is None:
             continue
         count, width, stride = _matrix(t, name)
         _refuse_unless(width == dim and t.dtype == grad_out.dtype,
-                       f"{name} and grad_out differ in dim or type")
+                       "rows, grad_rows and grad_out differ in dim or type")
         _refuse_unless(num_rows in (None, count), "rows and grad_rows differ in rows")
         num_rows = count
-        if name == "rows":
+        if t is rows:
             rows_stride = stride
-        else:
+        if t is grad_rows:
             grad_stride = stride
-        tensors.append(t)
     if positions is not None:
         p, slots = _positions(n, positions)
-        tensors.append(positions)
     else:
         p, slots = None, _by_place(slots, weights, grad_weights)
     w_kind = 0
     for t, name in ((weights, "weights"), (grad_weights, "grad_weights")):
         if t is not None:
             w_kind = _weights(t, name, n, slots, kind)
-            tensors.append(t)
     if weights is not None and grad_weights is not None:
         _refuse_unless(weights.dtype == grad_weights.dtype,
                        "weights and grad_weights differ in type")
-    index = _one_device(tensors)
+    index = _one_device(grad_out, rows, grad_rows, positions, weights, grad_weights)
     _call_on(index, stream, lib().hkv_combine_rows_backward, n, slots, dim, kind, _ptr(rows),
              rows_stride, num_rows, p, _ptr(weights), w_kind, grad_out.data_ptr(), out_stride,
              _ptr(grad_rows), grad_stride, _ptr(grad_weights))
