@@ -1048,7 +1048,9 @@ class PagePool:
     page. refs (int32 [pages]: 0 is a free page), table (int32 [rows,
     max_pages]: page numbers of each sequence) and lengths (int32 [rows]:
     tokens) are the pool's state; they are made here, empty, from num_rows and
-    max_pages unless given. Calls on one pool must be ordered by the caller.
+    max_pages unless given. Scratch comes from `allocator`, PyTorch's caching
+    allocator when None (see HashTable.init). Calls on one pool must be ordered by
+    the caller.
 
     With a HashTable of page numbers as its index, hold(n, pages, 1) keeps the
     pages that the index names in use, and hold(n, evicted_values, -1) lets go
@@ -1112,11 +1114,11 @@ class PagePool:
         o.planes = (_P * max(len(planes), 1))(*[t.data_ptr() for t in planes])
         o.page_bytes = (_U64 * max(len(planes), 1))(
             *[t.numel() // num_pages * t.element_size() for t in planes])
-        self._alloc_cbs = None if allocator is None else _allocator_callbacks(allocator)
+        # (kept alive with the pool)
+        self._alloc_cbs = _allocator_callbacks(allocator or TorchAllocator(self._index))
         h = ctypes.c_void_p()
-        _check(lib().hkv_pages_create(
-            ctypes.byref(o), None if allocator is None else ctypes.byref(self._alloc_cbs),
-            ctypes.byref(h)))
+        _check(lib().hkv_pages_create(ctypes.byref(o), ctypes.byref(self._alloc_cbs),
+                                      ctypes.byref(h)))
         self._h = h.value
 
     def close(self) -> None:
