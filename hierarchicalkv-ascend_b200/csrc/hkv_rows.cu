@@ -258,10 +258,16 @@ __global__ void __launch_bounds__(kSortThreads, 4)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr uint32_t kTile = kSortThreads * kItems;
   after_previous();
+  const uint32_t first = blockIdx.x * tiles_per_block;
+  int id[kItems];  // of the first tile: in flight while the starts are summed
+#pragma unroll
+  for (int it = 0; it < kItems; it++)
+    id[it] = load_group<Id>(groups, first * kTile + (warp * kItems + it) * 32 + lane, n, num_groups);
   if (totals == nullptr) {  // a warp per group sums the blocks' counts
     for (uint32_t g = warp; g < num_groups; g += kSortWarps) {
       const uint32_t* c = counts + static_cast<uint64_t>(g) * gridDim.x;
       uint32_t before = 0, all = 0;
+#pragma unroll 8
       for (uint32_t b = lane; b < gridDim.x; b += 32) {
         const uint32_t v = c[b];
         all += v;
@@ -282,7 +288,6 @@ __global__ void __launch_bounds__(kSortThreads, 4)
     }
     __syncthreads();
   }
-  const uint32_t first = blockIdx.x * tiles_per_block;
 
   // start of each group, over contiguous runs of groups per thread
   const uint32_t per = (num_groups + kSortThreads - 1) / kSortThreads;
@@ -305,10 +310,9 @@ __global__ void __launch_bounds__(kSortThreads, 4)
   for (uint32_t t = 0; t < tiles_per_block; t++) {
     const uint32_t base = (first + t) * kTile + warp * 32 * kItems + lane;
     if ((first + t) * kTile >= n) break;
-    int id[kItems];
     uint32_t rank[kItems];
 #pragma unroll
-    for (int it = 0; it < kItems; it++)
+    for (int it = 0; it < kItems && t > 0; it++)
       id[it] = load_group<Id>(groups, base + it * 32, n, num_groups);
     for (uint32_t k = threadIdx.x; k < num_groups * kSortWarps; k += kSortThreads) cnt[k] = 0;
     __syncthreads();
