@@ -529,7 +529,7 @@ int hkv_combine_rows(size_t n, size_t slots, size_t dim, int value_type,
  * grad_rows[positions[i]] = weights[i] * grad_out[t], rows that no place has
  * as they were; grad_weights[i] (weight_type) = the inner product of
  * grad_out[t] and rows[positions[i]], summed in float32 in an order that
- * depends on the sizes only, 0 for a place without a row. Every row is the
+ * depends on sizes and alignment only, 0 for a place without a row. Every row is the
  * row of one place at most, as hkv_group_tokens makes them; a row of several
  * places would get the gradient of one of them, or a mixture. rows is read
  * for grad_weights only. */

@@ -401,6 +401,52 @@ def test_captured_and_replayed():
         near(grads[1], square.expand(n, slots), dim * U * square.expand(n, slots))
 
 
+def test_captured_between_branches_copies_and_other_kernels():
+    """Nodes before and after the calls that are no kernels of this library, and
+    two streams that join: each call sees what came before it."""
+    n, groups = 70000, 32
+    source = torch.zeros(n, dtype=torch.int32, device="cuda")
+    first, second = i32(n), i32(n)
+    out = [(i32(groups + 1), i32(n), i32(n)) for _ in range(3)]
+    moved, pool_rows = torch.zeros((n, 1), device="cuda"), torch.zeros((n, 1), device="cuda")
+    side = torch.cuda.Stream()
+    H.group_tokens(n, source, groups, *out[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            second.copy_(source)
+            second.add_(1).remainder_(groups)
+            H.group_tokens(n, second, groups, *out[1])
+        first.copy_(source)  # a copy node, then the call
+        H.group_tokens(n, first, groups, *out[0])
+        main.wait_stream(side)
+        H.group_tokens(n, second, groups, *out[2])  # after the join
+        pool_rows.zero_()
+        H.dispatch_rows(n, source.view(torch.float32).view(n, 1), out[2][1].view(n, 1), pool_rows)
+        moved.copy_(pool_rows)
+    for seed in (5, 6):
+        source.copy_(torch.randint(0, groups, (n,), generator=seeded(seed), device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        later = (source + 1) % groups
+        for ids, got in ((source, out[0]), (later, out[1]), (later, out[2])):
+            want = sorted_reference(ids, groups)
+            assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip(got, want))
+        order = out[2][2].long()
+        assert torch.equal(moved.view(torch.int32).view(-1), source[order])
+
+
+def test_default_stream_by_its_number():
+    ids = torch.randint(0, 50, (6000,), device="cuda")
+    out = i32(51), i32(6000), i32(6000)
+    H.group_tokens(6000, ids, 50, *out, stream=0)
+    torch.cuda.synchronize()
+    assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip(out, sorted_reference(ids, 50)))
+
+
 def test_same_bits_every_time():
     g = seeded(8)
     n, slots, dim = 500, 6, 200
