@@ -515,41 +515,6 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// kVec elements of a row: 16 bytes where rows are aligned to that, else one. In
-// registers a wide pack stays in its four words until it is used (unpacked at
-// once, 58 registers held a combine kernel at half the warps of an SM).
-template <class T, int kVec>
-struct Pack {
-  T v;
-  __device__ __forceinline__ void unpack(float (&f)[kVec]) const { f[0] = to_float(v); }
-  __device__ __forceinline__ void pack(const float (&f)[kVec]) { v = from_float<T>(f[0]); }
-  __device__ __forceinline__ void load(const T* p) { v = *p; }
-  __device__ __forceinline__ void load_once(const T* p) { v = *p; }
-  __device__ __forceinline__ void store_once(T* p) const { *p = v; }
-};
-
-// Rows are read and written once: they need not stay in the caches.
-struct WidePack {
-  uint4 v;
-  __device__ __forceinline__ void load(const void* p) { v = *static_cast<const uint4*>(p); }
-  __device__ __forceinline__ void load_once(const void* p) {
-    v = __ldcs(static_cast<const uint4*>(p));
-  }
-  __device__ __forceinline__ void store_once(void* p) const { __stcs(static_cast<uint4*>(p), v); }
-};
-
-template <>
-struct Pack<float, 4> : WidePack {
-  __device__ __forceinline__ void unpack(float (&f)[4]) const {
-    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
-    f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
-  }
-  __device__ __forceinline__ void pack(const float (&f)[4]) {
-    v = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                   __float_as_uint(f[3]));
-  }
-};
-
 // the two halves of a word
 __device__ __forceinline__ float2 unpack2(uint32_t u, __nv_bfloat16) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
@@ -566,20 +531,60 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
   return reinterpret_cast<const uint32_t&>(h);
 }
 
-template <class T>
-struct Pack<T, 8> : WidePack {
-  __device__ __forceinline__ void unpack(float (&f)[8]) const {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// kVec elements of a row, 16 bytes where addresses, strides and rows allow, else 8,
+// 4 or one element. In registers a pack stays in its words until it is used
+// (unpacked at once, 58 registers held a combine kernel at half the warps of an
+// SM). Rows are read and written once: they need not stay in the caches.
+template <class T, int kVec>
+struct Pack {
+  static constexpr int kBytes = sizeof(T) * kVec, kWords = kBytes / 4;
+  using Raw = typename Word<kBytes>::type;
+  union {
+    Raw raw;
+    uint32_t word[kWords ? kWords : 1];
+  };
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const Raw*>(p); }
+  __device__ __forceinline__ void load_once(const T* p) {
+    raw = __ldcs(reinterpret_cast<const Raw*>(p));
+  }
+  __device__ __forceinline__ void store_once(T* p) const { __stcs(reinterpret_cast<Raw*>(p), raw); }
+  __device__ __forceinline__ void unpack(float (&f)[kVec]) const {
+    if constexpr (kWords == 0) {
+      f[0] = to_float(reinterpret_cast<const T&>(raw));
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const float2 h = unpack2(w[k], T{});
-      f[2 * k] = h.x;
-      f[2 * k + 1] = h.y;
+      for (int k = 0; k < kWords; k++) f[k] = __uint_as_float(word[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kWords; k++) {
+        const float2 h = unpack2(word[k], T{});
+        f[2 * k] = h.x;
+        f[2 * k + 1] = h.y;
+      }
     }
   }
-  __device__ __forceinline__ void pack(const float (&f)[8]) {
-    v = make_uint4(pack2(f[0], f[1], T{}), pack2(f[2], f[3], T{}), pack2(f[4], f[5], T{}),
-                   pack2(f[6], f[7], T{}));
+  __device__ __forceinline__ void pack(const float (&f)[kVec]) {
+    if constexpr (kWords == 0) {
+      const T t = from_float<T>(f[0]);
+      raw = reinterpret_cast<const Raw&>(t);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < kWords; k++) word[k] = __float_as_uint(f[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kWords; k++) word[k] = pack2(f[2 * k], f[2 * k + 1], T{});
+    }
+  }
+};
+
+// Weights are float32 or of the rows' type T; null stands for ones.
+template <class T>
+struct Weights {
+  const void* p;
+  bool wide;
+  __device__ __forceinline__ float at(uint64_t i) const {
+    if (p == nullptr) return 1.f;
+    return wide ? static_cast<const float*>(p)[i] : to_float(static_cast<const T*>(p)[i]);
   }
 };
 
@@ -640,14 +645,14 @@ __global__ void __launch_bounds__(kRowThreads, 6)
 // bound by memory, 8192 tokens of 8 KB with eight rows each, 1131 MB, in 176 us
 // (6.4 TB/s). A warp per place, which reads the token's gradient for each of its
 // slots, took 195 us, and 379 with four packs in flight.
-template <class T, class W, int kVec, int kTeam>
+template <class T, int kVec, int kTeam>
 __global__ void __launch_bounds__(kRowThreads, 4)
     combine_backward_kernel(uint32_t n, uint32_t slots, uint32_t packs,
                             const T* __restrict__ rows, uint64_t rows_stride, uint32_t num_rows,
-                            const int32_t* __restrict__ positions, const W* __restrict__ weights,
+                            const int32_t* __restrict__ positions, Weights<T> weights,
                             const T* __restrict__ grad_out, uint64_t grad_out_stride,
                             T* __restrict__ grad_rows, uint64_t grad_rows_stride,
-                            W* __restrict__ grad_weights) {
+                            void* __restrict__ grad_weights) {
   using P = Pack<T, kVec>;
   constexpr int kAhead = 4, kWarps = kTeam / 32;
   __shared__ float sums[2][kAhead][kRowThreads / 32];
@@ -665,7 +670,7 @@ __global__ void __launch_bounds__(kRowThreads, 4)
       row[a] = !on         ? ~0u
                : positions ? static_cast<uint32_t>(positions[place + k + a])
                            : static_cast<uint32_t>(place + k + a);
-      w[a] = weights && row[a] < num_rows ? to_float(weights[place + k + a]) : 1.f;
+      w[a] = row[a] < num_rows ? weights.at(place + k + a) : 1.f;
       dot[a] = 0.f;
     }
     for (uint32_t p = lane; t < n && p < packs; p += kTeam) {
@@ -721,7 +726,12 @@ __global__ void __launch_bounds__(kRowThreads, 4)
     if (t < n && lane == 0) {
 #pragma unroll
       for (int a = 0; a < kAhead; a++)
-        if (k + a < slots) grad_weights[place + k + a] = from_float<W>(dot[a]);
+        if (k + a < slots) {
+          if (weights.wide)
+            static_cast<float*>(grad_weights)[place + k + a] = dot[a];
+          else
+            static_cast<T*>(grad_weights)[place + k + a] = from_float<T>(dot[a]);
+        }
     }
   }
 }
@@ -822,30 +832,36 @@ void launch_combine(const RowShape& r, const void* rows, uint64_t rows_stride, s
   });
 }
 
-template <class T, class W, int kVec, int kTeam>
+template <class T, int kVec, int kTeam>
 void launch_backward(const RowShape& r, const void* rows, uint64_t rows_stride, size_t num_rows,
-                     const int32_t* positions, const void* weights, const void* grad_out,
+                     const int32_t* positions, Weights<T> weights, const void* grad_out,
                      uint64_t grad_out_stride, void* grad_rows, uint64_t grad_rows_stride,
                      void* grad_weights, cudaStream_t s) {
-  launch(combine_backward_kernel<T, W, kVec, kTeam>, blocks_for(r.n * kTeam), kRowThreads, 0, s, 1,
+  launch(combine_backward_kernel<T, kVec, kTeam>, blocks_for(r.n * kTeam), kRowThreads, 0, s, 1,
          static_cast<uint32_t>(r.n), static_cast<uint32_t>(r.slots),
          static_cast<uint32_t>(r.dim / kVec), static_cast<const T*>(rows), rows_stride,
-         static_cast<uint32_t>(num_rows), positions, static_cast<const W*>(weights),
+         static_cast<uint32_t>(num_rows), positions, weights,
          static_cast<const T*>(grad_out), grad_out_stride, static_cast<T*>(grad_rows),
-         grad_rows_stride, static_cast<W*>(grad_weights));
+         grad_rows_stride, grad_weights);
 }
 
-// calls f with the row type and the weight type as values of those types
+// Calls f with the row type as a value and the elements of a pack as a constant:
+// the widest that `bytes`, a power of two, allows.
 template <class F>
-void with_types(int value_type, int weight_type, F f) {
+void with_packs(int value_type, uint32_t bytes, F f) {
   auto pick = [&](auto t) {
-    if (weight_type == value_type)
-      f(t, t);
+    constexpr int kSize = sizeof(t);
+    if (bytes == 16)
+      f(t, std::integral_constant<int, 16 / kSize>{});
+    else if (bytes == 8)
+      f(t, std::integral_constant<int, 8 / kSize>{});
+    else if (bytes == 4 && kSize < 4)
+      f(t, std::integral_constant<int, 2>{});
     else
-      f(t, float{});
+      f(t, std::integral_constant<int, 1>{});
   };
   if (value_type == HKV_VALUE_F32)
-    f(float{}, float{});
+    pick(float{});
   else if (value_type == HKV_VALUE_F16)
     pick(__half{});
   else
@@ -943,17 +959,18 @@ int hkv_combine_rows(size_t n, size_t slots, size_t dim, int value_type, const v
   if (positions) hkvb::require(positions, 4, "positions");
   if (weights) hkvb::require(weights, hkvb::type_bytes(wt), "weights");
   hkvb::require(out, r.bytes, "out");
-  const bool wide =
-      hkvb::word_bytes({rows, out}, {dim * r.bytes, rs * r.bytes, os * r.bytes}) == 16;
-  hkvb::with_types(value_type, wt, [&](auto t, auto w) {
+  const uint32_t bytes =
+      hkvb::word_bytes({rows, out}, {dim * r.bytes, rs * r.bytes, os * r.bytes});
+  hkvb::with_packs(value_type, bytes, [&](auto t, auto vec) {
     using T = decltype(t);
-    using W = decltype(w);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (wide)
-      hkvb::launch_combine<T, W, 16 / sizeof(T)>(r, rows, rs, num_rows, positions, weights, out,
-                                                 os, s);
+    auto go = [&](auto w) {
+      hkvb::launch_combine<T, decltype(w), decltype(vec)::value>(
+          r, rows, rs, num_rows, positions, weights, out, os, static_cast<cudaStream_t>(stream));
+    };
+    if (wt == HKV_VALUE_F32)
+      go(float{});
     else
-      hkvb::launch_combine<T, W, 1>(r, rows, rs, num_rows, positions, weights, out, os, s);
+      go(t);
   });
   HKV_API_END
 }
@@ -978,33 +995,35 @@ int hkv_combine_rows_backward(size_t n, size_t slots, size_t dim, int value_type
     if (num_rows > 0) hkvb::require(rows, r.bytes, "rows");
     hkvb::require(grad_weights, hkvb::type_bytes(wt), "grad_weights");
   }
-  const bool wide = hkvb::word_bytes({grad_weights ? rows : nullptr, grad_out, grad_rows},
-                                     {dim * r.bytes, rs * r.bytes, gs * r.bytes,
-                                      ys * r.bytes}) == 16;
-  hkvb::with_types(value_type, wt, [&](auto t, auto w) {
+  const uint32_t bytes = hkvb::word_bytes({grad_weights ? rows : nullptr, grad_out, grad_rows},
+                                          {dim * r.bytes, rs * r.bytes, gs * r.bytes,
+                                           ys * r.bytes});
+  hkvb::with_packs(value_type, bytes, [&](auto t, auto vec) {
     using T = decltype(t);
-    using W = decltype(w);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    auto go = [&](auto vec, auto team) {
-      hkvb::launch_backward<T, W, decltype(vec)::value, decltype(team)::value>(
-          r, rows, rs, num_rows, positions, weights, grad_out, gs, grad_rows, ys, grad_weights,
-          s);
+    constexpr int kVec = decltype(vec)::value;
+    auto go = [&](auto team) {
+      hkvb::launch_backward<T, kVec, decltype(team)::value>(
+          r, rows, rs, num_rows, positions, hkvb::Weights<T>{weights, wt == HKV_VALUE_F32},
+          grad_out, gs, grad_rows, ys, grad_weights, static_cast<cudaStream_t>(stream));
     };
-    auto pick = [&](auto vec) {  // the smallest team that covers a row, 256 at most
-      const size_t packs = dim / decltype(vec)::value;
-      if (packs <= 8)
-        go(vec, std::integral_constant<int, 8>{});
-      else if (packs <= 32)
-        go(vec, std::integral_constant<int, 32>{});
-      else if (packs <= 128)
-        go(vec, std::integral_constant<int, 128>{});
-      else
-        go(vec, std::integral_constant<int, 256>{});
-    };
-    if (wide)
-      pick(std::integral_constant<int, 16 / sizeof(T)>{});
+    // Few idle threads and few steps over a row: measured for 250 MB of rows (us
+    // with teams of 16, 32, 64, 128, 256): 25 packs 143 137 190 - -, 52 packs 110
+    // 105 121 166 274, 84 packs 109 100 116 126 180, 170 packs 117 103 97 111 119,
+    // 333 packs 122 112 102 96 108, 512 packs 109 96 90 91 88, 1024 packs 157 110
+    // 94 89 90.
+    const size_t packs = dim / kVec;
+    if (packs <= 8)
+      go(std::integral_constant<int, 8>{});
+    else if (packs <= 16)
+      go(std::integral_constant<int, 16>{});
+    else if (packs <= 96)
+      go(std::integral_constant<int, 32>{});
+    else if (packs <= 288)
+      go(std::integral_constant<int, 64>{});
+    else if (packs < 512)
+      go(std::integral_constant<int, 128>{});
     else
-      pick(std::integral_constant<int, 1>{});
+      go(std::integral_constant<int, 256>{});
   });
   HKV_API_END
 }
