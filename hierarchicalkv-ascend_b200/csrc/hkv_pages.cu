@@ -103,9 +103,11 @@ __global__ void __launch_bounds__(kCopyThreads)
 // it reads its sources and what its destinations held (counts + 1 and - 1), then
 // writes. Lengths are read by all blocks and written by the last one to have
 // read them. The sums of counts do not depend on the order of their atomics.
-// Bound by latency: eight rows of 21 pages in 5 us. Its blocks are few (one for
-// eight columns): at 960 rows of 512 columns it took 18 us and the two launches
-// below 6.4 + 6.2, so it serves lists of 32768 entries at most.
+// Bound by latency. Its blocks are few, one for eight columns, and each goes over
+// the whole list: in a graph 8 rows of 64 columns take 3.5 us, in the two launches
+// below 4.2, 64 rows of 64 columns 3.8 / 4.2, 200 of 128 5.4 / 4.5, 960 of 512
+// 12.8 / 9.9, one of 16384 18.5 / 6.9. It serves 16384 entries of 1024 columns at
+// most (the second launch costs the host 2 us).
 
 constexpr uint32_t kForkColumns = 8;  // a sector of a row
 constexpr uint32_t kForkColumnThreads = 1024;
@@ -646,7 +648,7 @@ class OnDevice {
 class PagesImpl {
   static constexpr int kMostShared = 200 * 1024;
   static constexpr uint32_t kOneLaunchChunks = 256, kOneLaunchMoves = 1024;
-  static constexpr size_t kOneLaunchEntries = 1 << 15;
+  static constexpr size_t kOneLaunchEntries = 1 << 14, kOneLaunchColumns = 1 << 10;
   // Blocks of a move per SM: 8 stay resident and take 12 units each one after
   // the other (90 us for 472 MB), 32 hide a unit's chain of loads behind the
   // next block's (81), 256 mostly find nothing left to do (99).
@@ -720,7 +722,8 @@ class PagesImpl {
     const bool many_rows = o.num_rows * 4ull > kMostShared;
     const size_t a_owners = part(many_rows ? o.num_rows * 4ull * kPlanBlocks : 0);
     // entries of forked rows, for lists that take two launches
-    const bool stages = fork_smem(o.num_rows, o.num_rows) > kMostShared ||
+    const bool stages = o.max_pages > kOneLaunchColumns ||
+                        fork_smem(o.num_rows, o.num_rows) > kMostShared ||
                         static_cast<size_t>(o.num_rows) * o.max_pages > kOneLaunchEntries;
     const size_t a_staged =
         part(stages ? static_cast<size_t>(o.num_rows) * o.max_pages * 4 : 0);
@@ -781,7 +784,8 @@ class PagesImpl {
     check_list(dst, "dst");
     OnDevice on(device_);
     const size_t smem = fork_smem(view_.num_rows, n);
-    if (n * view_.max_pages <= kOneLaunchEntries && smem <= kMostShared) {
+    if (view_.max_pages <= kOneLaunchColumns && n * view_.max_pages <= kOneLaunchEntries &&
+        smem <= kMostShared) {
       launch(fork_columns_kernel, (view_.max_pages + kForkColumns - 1) / kForkColumns,
              kForkColumnThreads, smem, s, 1, view_, static_cast<uint32_t>(n), src, dst, arrived_);
       return;

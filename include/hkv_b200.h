@@ -601,9 +601,9 @@ int hkv_pages_fork(hkv_pages* pool, size_t n, const int32_t* src,
                    const int32_t* dst, void* stream);
 
 /* Row rows[i] gets the length lengths[i] (tokens). Growing takes free pages;
- * where its last page is only partly filled and shared, the row first gets a
- * copy of that page, so that what is written behind the old length is seen by
- * this row alone. Shrinking gives pages back. Free pages are those that are
+ * where its last page is only partly filled and shared (as the call begins),
+ * the row first gets a copy of that page, so that what is written behind the
+ * old length is seen by this row alone. Shrinking gives pages back. Free pages are those that are
  * free as the call begins; they are handed out lowest number first, to the
  * entries in their order (an entry's copy first, then its new pages).
  * status[i] (nullable) tells whether the entry was served. One that was not
