@@ -235,7 +235,8 @@ __global__ void __launch_bounds__(kForkThreads)
 
 // ---- free and hold ----------------------------------------------------------
 
-__global__ void __launch_bounds__(256) free_rows_kernel(PoolView v, const int32_t* rows) {
+// a block per row, of 256 threads, or 1024 where rows may be long
+__global__ void __launch_bounds__(1024) free_rows_kernel(PoolView v, const int32_t* rows) {
   after_previous();
   const uint32_t r = static_cast<uint32_t>(rows[blockIdx.x]);
   if (r >= v.num_rows) return;
@@ -328,40 +329,40 @@ struct Want {
   uint32_t first;  // place in the list of free pages, ~0: not served
 };
 
-// Chunk y of `chunks_at_once` of entry e: the first one also changes the table.
+// Share y of `shares` of entry e: its chunks of the page copy and its entries of the
+// table; the first one also writes what there is one of.
 template <int kBytes>
 __device__ __forceinline__ void resize_entry(const PlaneSet& planes, const PoolView& v,
                                              const Want* wants, const int32_t* free_list,
                                              bool* status, uint32_t e, uint32_t y,
-                                             uint32_t chunks_at_once, uint32_t tid) {
+                                             uint32_t shares, uint32_t tid) {
   const Want w = wants[e];
   const bool served = w.row >= 0 && w.first != ~0u;
   if (y == 0 && tid == 0 && status) status[e] = served;
   if (!served) return;
   const bool copied = w.shared >= 0;
-  if (y == 0) {
-    const uint32_t have = v.pages_of(w.old), want = v.pages_of(w.length);
-    int32_t* row = v.row(w.row);
-    for (uint32_t j = have + tid; j < want; j += kCopyThreads) {
-      const int32_t page = free_list[w.first + copied + j - have];
-      row[j] = page;
-      v.refs[page] = 1;
-    }
-    for (uint32_t j = want + tid; j < have; j += kCopyThreads) {
-      const int32_t page = row[j];
-      if (static_cast<uint32_t>(page) < v.num_pages) atomicSub(&v.refs[page], 1);
-    }
-    if (tid == 0) {
-      v.lengths[w.row] = w.length;
-      if (copied) {
-        row[have - 1] = free_list[w.first];
-        v.refs[free_list[w.first]] = 1;
-        atomicSub(&v.refs[w.shared], 1);
-      }
+  const uint32_t have = v.pages_of(w.old), want = v.pages_of(w.length);
+  const uint32_t at = y * kCopyThreads + tid, step = shares * kCopyThreads;
+  int32_t* row = v.row(w.row);
+  for (uint32_t j = have + at; j < want; j += step) {
+    const int32_t page = free_list[w.first + copied + j - have];
+    row[j] = page;
+    v.refs[page] = 1;
+  }
+  for (uint32_t j = want + at; j < have; j += step) {
+    const int32_t page = row[j];
+    if (static_cast<uint32_t>(page) < v.num_pages) atomicSub(&v.refs[page], 1);
+  }
+  if (at == 0) {
+    v.lengths[w.row] = w.length;
+    if (copied) {
+      row[have - 1] = free_list[w.first];
+      v.refs[free_list[w.first]] = 1;
+      atomicSub(&v.refs[w.shared], 1);
     }
   }
   if (copied)
-    for (uint32_t c = y; c < planes.chunks; c += chunks_at_once)
+    for (uint32_t c = y; c < planes.chunks; c += shares)
       copy_chunk<kBytes>(planes, c, w.shared, free_list[w.first], tid);
 }
 
@@ -385,7 +386,7 @@ __device__ __forceinline__ Want wanted(const PoolView& v, int32_t row, int32_t l
 }
 
 // owners: kPlanBlocks arrays of num_rows in global memory, null where one fits
-// shared memory. chunks_at_once: 0 leaves the changes to resize_apply_kernel.
+// shared memory. shares of an entry: 0 leaves the changes to resize_apply_kernel.
 // A list that fits the threads of a block, on a pool of one strip, is planned
 // by the first block alone.
 template <int kBytes>
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(kStripThreads)
     resize_plan_kernel(const __grid_constant__ PlaneSet planes, PoolView v, uint32_t n,
                        const int32_t* rows, const int32_t* lengths, uint32_t strips,
                        int32_t* owners, Want* wants, uint32_t* needs, int32_t* free_list,
-                       bool* status, uint32_t chunks_at_once) {
+                       bool* status, uint32_t shares) {
   extern __shared__ int32_t owner_smem[];
   __shared__ uint32_t shared[2];
   const uint32_t rank = cluster_rank();
@@ -480,9 +481,9 @@ __global__ void __launch_bounds__(kStripThreads)
   cluster_sync();
   const uint32_t team = (rank * kStripThreads + threadIdx.x) / kCopyThreads;
   constexpr uint32_t kTeams = kPlanBlocks * kStripThreads / kCopyThreads;
-  for (uint32_t u = team; u < n * chunks_at_once; u += kTeams)
-    resize_entry<kBytes>(planes, v, wants, free_list, status, u / chunks_at_once,
-                         u % chunks_at_once, chunks_at_once, threadIdx.x % kCopyThreads);
+  for (uint32_t u = team; u < n * shares; u += kTeams)
+    resize_entry<kBytes>(planes, v, wants, free_list, status, u / shares,
+                         u % shares, shares, threadIdx.x % kCopyThreads);
 }
 
 template <int kBytes>
@@ -647,7 +648,8 @@ class OnDevice {
 
 class PagesImpl {
   static constexpr int kMostShared = 200 * 1024;
-  static constexpr uint32_t kOneLaunchChunks = 256, kOneLaunchMoves = 1024;
+  static constexpr uint32_t kOneLaunchShares = 256, kOneLaunchMoves = 1024;
+  static constexpr uint32_t kPageStep = 1024;  // pages of a row that one share goes over
   static constexpr size_t kOneLaunchEntries = 1 << 14, kOneLaunchColumns = 1 << 10;
   // Blocks of a move per SM: 8 stay resident and take 12 units each one after
   // the other (90 us for 472 MB), 32 hide a unit's chain of loads behind the
@@ -804,20 +806,21 @@ class PagesImpl {
     check_list(lengths, "lengths");
     OnDevice on(device_);
     const uint32_t m = static_cast<uint32_t>(n);
-    // in one launch up to some copied chunks per team of threads
-    const uint32_t chunks = std::max(1u, planes_.chunks);
-    const bool one = static_cast<uint64_t>(m) * chunks <= kOneLaunchChunks;
-    const uint32_t at_once = one ? chunks : 0;
+    // shares of an entry: its copied chunks, or steps over its pages; in one launch
+    // up to some per team of threads
+    const uint32_t shares =
+        std::max({1u, planes_.chunks, (view_.max_pages + kPageStep - 1) / kPageStep});
+    const bool one = static_cast<uint64_t>(m) * shares <= kOneLaunchShares;
     const size_t smem = owners_ ? 0 : view_.num_rows * 4ull;
     with_width([&](auto width) {
       constexpr int kBytes = decltype(width)::value;
       launch(resize_plan_kernel<kBytes>, kPlanBlocks, kStripThreads, smem, s, kPlanBlocks, planes_,
-             view_, m, rows, lengths, strips_, owners_, wants_, needs_, list_, status, at_once);
+             view_, m, rows, lengths, strips_, owners_, wants_, needs_, list_, status, one ? shares : 0);
       if (one) return;
-      // blocks of an entry: as many as its page copy can use, few where there
-      // are entries enough to fill the device
+      // blocks of an entry: as many as it can use, few where there are entries
+      // enough to fill the device
       const uint32_t fill = std::max(1u, static_cast<uint32_t>(sm_count_) * 16 / m);
-      launch(resize_apply_kernel<kBytes>, dim3(m, std::min(chunks, fill)),
+      launch(resize_apply_kernel<kBytes>, dim3(m, std::min(shares, fill)),
              kCopyThreads, 0, s, 1, planes_, view_, wants_, list_, status);
     });
   }
@@ -827,7 +830,8 @@ class PagesImpl {
     if (n == 0) return;
     check_list(rows, "rows");
     OnDevice on(device_);
-    launch(free_rows_kernel, static_cast<uint32_t>(n), 256, 0, s, 1, view_, rows);
+    launch(free_rows_kernel, static_cast<uint32_t>(n), view_.max_pages > 1024 ? 1024 : 256, 0, s, 1,
+           view_, rows);
   }
 
   void hold(size_t n, const int32_t* pages, int delta, cudaStream_t s) {
