@@ -743,12 +743,16 @@ class PagesImpl {
     try {
       CUDA_TRY(cudaMemset(arrived_, 0, 4));
       CUDA_TRY(cudaDeviceSynchronize());
-      CUDA_TRY(cudaFuncSetAttribute(fork_columns_kernel,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
-      with_width([&](auto width) {
-        CUDA_TRY(cudaFuncSetAttribute(resize_plan_kernel<decltype(width)::value>,
+      // kernels that this pool may give more than 48 KB of shared memory
+      if (fork_smem(o.num_rows, o.num_rows) > 48 * 1024)
+        CUDA_TRY(cudaFuncSetAttribute(fork_columns_kernel,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
-      });
+      if (o.num_rows * 4ull > 48 * 1024)
+        with_width([&](auto width) {
+          CUDA_TRY(cudaFuncSetAttribute(resize_plan_kernel<decltype(width)::value>,
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        kMostShared));
+        });
     } catch (...) {
       mem_.free_device(scratch_);
       throw;
