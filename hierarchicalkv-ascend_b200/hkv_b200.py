@@ -789,7 +789,7 @@ class _Torch:
         import torch as t
 
         self.torch = t
-        self.int32, self.bool = t.int32, t.bool
+        self.int32, self.uint8, self.bool = t.int32, t.uint8, t.bool
         self.ids = {t.int32: 0, t.int64: 1}
         self.rows = {t.float32: 0, t.float16: 1, t.bfloat16: 2, t.float64: 3, t.int32: 4,
                      t.uint32: 4, t.int16: 5, t.uint16: 5, t.int8: 6, t.uint8: 6, t.int64: 7,
@@ -815,66 +815,103 @@ def _refuse_unless(ok, message):
         raise HkvException(message)
 
 
-def _matrix(t, name, n=0):
-    """(rows, dim, elements from row to row) of a 2-D tensor whose rows are
-    contiguous and do not overlap."""
+# Checks of one tensor each, in one step where it is as it should be; what is wrong
+# with one that is not is looked for after that. `index`: the device to be on.
+
+def _matrix(t, name, n, index, dim=None, dtype=None):
+    """(rows, dim, elements from row to row, address) of a 2-D tensor whose rows
+    are contiguous and do not overlap."""
     shape, stride = t.shape, t.stride()
-    if len(shape) == 2:
-        rows, dim = shape
-        if n <= rows and stride[0] >= dim > 0 and stride[1] == 1:
-            return rows, dim, stride[0]
+    if (len(shape) == 2 and stride[1] == 1 and n <= shape[0] and stride[0] >= shape[1] > 0
+            and (dtype is None or t.dtype is dtype and shape[1] == dim)
+            and t.get_device() == index):
+        return shape[0], shape[1], stride[0], t.data_ptr()
     _refuse_unless(len(shape) == 2, f"{name} must have two dimensions")
+    rows, width = shape
     _refuse_unless(n <= rows, f"{name} has {rows} rows, fewer than {n}")
-    _refuse_unless(dim > 0, f"{name} has empty rows")
-    _refuse_unless(stride[1] == 1 or dim == 1, f"the rows of {name} must be contiguous")
-    _refuse_unless(stride[0] >= dim or rows <= 1,
+    _refuse_unless(width > 0, f"{name} has empty rows")
+    _refuse_unless(stride[1] == 1 or width == 1, f"the rows of {name} must be contiguous")
+    _refuse_unless(stride[0] >= width or rows <= 1,
                    f"the rows of {name} overlap (an expanded tensor?)")
-    return rows, dim, max(stride[0], dim)
+    _refuse_unless(dtype is None or t.dtype == dtype, f"{name} must be {dtype}, not {t.dtype}")
+    _refuse_unless(dim is None or width == dim, f"{name} must have rows of {dim}, not {width}")
+    _refuse_unless(t.get_device() == index, "the tensors are on different devices")
+    return rows, width, max(stride[0], width), t.data_ptr()
 
 
-def _list(t, name, n, dtype):
-    """A contiguous tensor of at least n elements of one dtype."""
-    if t.dtype is dtype and t.numel() >= n and t.is_contiguous():
+def _list(t, name, n, index, dtype):
+    """Address of a contiguous tensor of at least n elements of one dtype."""
+    if (t.dtype is dtype and t.is_contiguous() and t.numel() >= n
+            and t.get_device() == index):
         return t.data_ptr()
     _refuse_unless(t.dtype == dtype, f"{name} must be {dtype}, not {t.dtype}")
     _refuse_unless(t.numel() >= n, f"{name} has {t.numel()} elements, fewer than {n}")
-    raise HkvException(f"{name} must be contiguous")
+    _refuse_unless(t.is_contiguous(), f"{name} must be contiguous")
+    raise HkvException(f"{name} is on another device")
 
 
-def _one_device(*tensors):
-    """Index of the CUDA device that all the tensors (or None) are on."""
-    index = tensors[0].get_device()
+def _per_place(t, name, n, index, slots=None):
+    """Address of a contiguous [tokens, slots] tensor with at least n tokens."""
+    shape = t.shape
+    if (len(shape) == 2 and n <= shape[0] and t.is_contiguous() and t.get_device() == index
+            and shape[1] > 0 and (slots is None or slots == shape[1])):
+        return t.data_ptr(), shape[1]
+    _refuse_unless(len(shape) == 2 and shape[1] > 0, f"{name} must be [tokens, slots]")
+    _refuse_unless(n <= shape[0], f"{name} has {shape[0]} tokens, fewer than {n}")
+    _refuse_unless(t.is_contiguous(), f"{name} must be contiguous")
+    _refuse_unless(slots in (None, shape[1]), f"{name} must have {slots} slots, not {shape[1]}")
+    raise HkvException(f"{name} is on another device")
+
+
+def _positions(t, n, index):
+    """(address, slots) of the int32 positions [tokens, slots]."""
+    if t.dtype is not _TORCH.int32:
+        raise HkvException(f"positions must be int32, not {t.dtype}")
+    return _per_place(t, "positions", n, index)
+
+
+def _weights(t, name, n, index, slots, kind):
+    """(address, value type) of weights of float32 or of the rows' type."""
+    got = _TORCH.rows.get(t.dtype)
+    if got != 0 and got != kind:
+        raise HkvException(f"{name} must be float32 or of the rows' type, not {t.dtype}")
+    return _per_place(t, name, n, index, slots)[0], got
+
+
+def _by_place(slots, *shaped):
+    """Slots of a call without positions: as told, else those of the weights."""
+    for t in shaped:
+        if t is not None and slots is None:
+            slots = t.shape[-1]
+    _refuse_unless(slots is not None and slots > 0,
+                   "without positions and weights, slots must be given")
+    return slots
+
+
+def _row_type(t):
+    """(value type, dtype, device index) of a tensor of rows."""
+    dtype = t.dtype
+    kind = (_TORCH or _torch()).rows.get(dtype)
+    if kind is None:
+        raise HkvException(f"rows of {dtype} are not supported")
+    return kind, dtype, t.get_device()
+
+
+def _call_on(index, stream, fn, n, *args):
+    """fn(n, *args, stream) with device `index` current."""
+    if n < 0:
+        raise HkvException("n must not be negative")
     if index < 0:
         raise HkvException("the tensors must be on a CUDA device")
-    for t in tensors:
-        if t is not None and t.get_device() != index:
-            raise HkvException("the tensors are on different devices")
-    return index
-
-
-def _call_on(index, stream, fn, *args):
-    """fn(*args, stream) with device `index` current."""
     t = _TORCH
     stream = t.stream(index) if stream is None else _stream(stream)
     if t.device() == index:
-        status = fn(*args, stream)
+        status = fn(n, *args, stream)
     else:
         with t.torch.cuda.device(index):
-            status = fn(*args, stream)
+            status = fn(n, *args, stream)
     if status:
         _check(status)
-
-
-def _row_kind(dtype):
-    kind = _torch().rows.get(dtype)
-    if kind is None:
-        raise HkvException(f"rows of {dtype} are not supported")
-    return kind
-
-
-def _not_negative(n):
-    if n < 0:
-        raise HkvException("n must not be negative")
 
 
 def group_workspace(n: int, num_groups: int) -> int:
@@ -896,39 +933,27 @@ def group_tokens(n, groups, num_groups, offsets, positions, order=None, workspac
     uint8 tensor of group_workspace(n, num_groups) bytes, allocated here when
     None; calls that may overlap need their own."""
     torch = _torch()
-    _not_negative(n)
-    ids = torch.ids.get(groups.dtype)
+    ids, index = torch.ids.get(groups.dtype), groups.get_device()
     if ids is None:
         raise HkvException(f"groups must be int32 or int64, not {groups.dtype}")
-    g = _list(groups, "groups", n, groups.dtype)
-    p = _list(positions, "positions", n, torch.int32)
-    f = _list(offsets, "offsets", num_groups + 1, torch.int32)
-    r = None if order is None else _list(order, "order", n, torch.int32)
-    index = _one_device(groups, positions, offsets, order, workspace)
+    g = _list(groups, "groups", n, index, groups.dtype)
+    p = _list(positions, "positions", n, index, torch.int32)
+    f = _list(offsets, "offsets", num_groups + 1, index, torch.int32)
+    r = None if order is None else _list(order, "order", n, index, torch.int32)
     if workspace is None:
         size = group_workspace(n, num_groups)
+        _refuse_unless(index >= 0, "the tensors must be on a CUDA device")
         cuda = torch.torch.cuda
         if isinstance(stream, int):
             stream = cuda.ExternalStream(stream, index)
         # from the pool of the stream that uses it
         with cuda.stream(stream or cuda.current_stream(index)):
-            workspace = torch.torch.empty(size, dtype=torch.torch.uint8, device=groups.device)
+            workspace = torch.torch.empty(size, dtype=torch.uint8, device=groups.device)
+        scratch = workspace.data_ptr()
     else:
-        size = workspace.nbytes
-        if not workspace.is_contiguous():
-            raise HkvException("workspace must be contiguous")
-    _call_on(index, stream, lib().hkv_group_tokens, n, g, ids, num_groups, f, p, r,
-             workspace.data_ptr(), size)
-
-
-def _positions(n, positions):
-    """(address, slots) of the int32 positions [tokens, slots]."""
-    shape = positions.shape
-    if len(shape) != 2 or shape[1] == 0:
-        raise HkvException("positions must be [tokens, slots]")
-    if n > shape[0]:
-        raise HkvException(f"positions has {shape[0]} tokens, fewer than {n}")
-    return _list(positions, "positions", 0, _TORCH.int32), shape[1]
+        size = workspace.numel()
+        scratch = _list(workspace, "workspace", 0, index, torch.uint8)
+    _call_on(index, stream, lib().hkv_group_tokens, n, g, ids, num_groups, f, p, r, scratch, size)
 
 
 def dispatch_rows(n, x, positions, rows, stream=None):
@@ -936,37 +961,12 @@ def dispatch_rows(n, x, positions, rows, stream=None):
     x: [tokens, dim], positions: int32 [tokens, slots], rows: [rows, dim]; a
     position outside rows is passed over and rows that no place has stay as
     they were. The gradient: combine_rows(n, grad_rows, positions, None, grad_x)."""
-    _not_negative(n)
-    _, dim, x_stride = _matrix(x, "x", n)
-    num_rows, width, rows_stride = _matrix(rows, "rows")
-    kind = _row_kind(x.dtype)
-    if width != dim or rows.dtype is not x.dtype:
-        raise HkvException("x and rows differ in dim or type")
-    p, slots = _positions(n, positions)
-    index = _one_device(x, positions, rows)
-    _call_on(index, stream, lib().hkv_dispatch_rows, n, slots, dim, kind, x.data_ptr(),
-             x_stride, p, num_rows, rows.data_ptr(), rows_stride)
-
-
-def _weights(weights, name, n, slots, kind):
-    shape, got = weights.shape, _TORCH.rows.get(weights.dtype)
-    if (len(shape) == 2 and shape[1] == slots and shape[0] >= n and weights.is_contiguous()
-            and (got == 0 or got == kind)):
-        return got
-    _refuse_unless(len(shape) == 2 and shape[1] == slots and shape[0] >= n,
-                   f"{name} must be [tokens, slots]")
-    _refuse_unless(weights.is_contiguous(), f"{name} must be contiguous")
-    raise HkvException(f"{name} must be float32 or of the rows' type")
-
-
-def _by_place(slots, *shaped):
-    """Slots of a call without positions: as told, else those of the weights."""
-    for t in shaped:
-        if t is not None and slots is None:
-            slots = t.shape[-1]
-    _refuse_unless(slots is not None and slots > 0,
-                   "without positions and weights, slots must be given")
-    return slots
+    kind, dtype, index = _row_type(x)
+    _, dim, x_stride, x_at = _matrix(x, "x", n, index)
+    num_rows, _, rows_stride, rows_at = _matrix(rows, "rows", 0, index, dim, dtype)
+    p, slots = _positions(positions, n, index)
+    _call_on(index, stream, lib().hkv_dispatch_rows, n, slots, dim, kind, x_at, x_stride, p,
+             num_rows, rows_at, rows_stride)
 
 
 def combine_rows(n, rows, positions, weights, out, stream=None, slots=None):
@@ -976,23 +976,18 @@ def combine_rows(n, rows, positions, weights, out, stream=None, slots=None):
     out: [tokens, dim]. positions None: the row of place (t, s) is t * slots +
     s (what find wrote for the keys of n tokens), with slots as given or those
     of weights. Summed in float32, rounded once."""
-    _not_negative(n)
-    num_rows, dim, rows_stride = _matrix(rows, "rows")
-    _, width, out_stride = _matrix(out, "out", n)
-    kind = _row_kind(rows.dtype)
-    if width != dim or out.dtype is not rows.dtype:
-        raise HkvException("rows and out differ in dim or type")
+    kind, dtype, index = _row_type(rows)
+    num_rows, dim, rows_stride, rows_at = _matrix(rows, "rows", 0, index)
+    _, _, out_stride, out_at = _matrix(out, "out", n, index, dim, dtype)
     if positions is not None:
-        p, slots = _positions(n, positions)
+        p, slots = _positions(positions, n, index)
     else:
         p, slots = None, _by_place(slots, weights)
     w, w_kind = None, 0
     if weights is not None:
-        w_kind = _weights(weights, "weights", n, slots, kind)
-        w = weights.data_ptr()
-    index = _one_device(rows, out, positions, weights)
-    _call_on(index, stream, lib().hkv_combine_rows, n, slots, dim, kind, rows.data_ptr(),
-             rows_stride, num_rows, p, w, w_kind, out.data_ptr(), out_stride)
+        w, w_kind = _weights(weights, "weights", n, index, slots, kind)
+    _call_on(index, stream, lib().hkv_combine_rows, n, slots, dim, kind, rows_at, rows_stride,
+             num_rows, p, w, w_kind, out_at, out_stride)
 
 
 def combine_rows_backward(n, rows, positions, weights, grad_out, grad_rows=None,
@@ -1003,40 +998,33 @@ def combine_rows_backward(n, rows, positions, weights, grad_out, grad_rows=None,
     without a row), either left out when None. Each row may be the row of one
     place only. rows may be None when grad_weights is. Without positions, slots
     as given or those of weights or grad_weights."""
-    _not_negative(n)
-    _, dim, out_stride = _matrix(grad_out, "grad_out", n)
-    kind = _row_kind(grad_out.dtype)
     _refuse_unless(rows is not None or grad_weights is None, "grad_weights needs rows")
+    kind, dtype, index = _row_type(grad_out)
+    _, dim, out_stride, out_at = _matrix(grad_out, "grad_out", n, index)
     if grad_rows is None and grad_weights is None:
         return
-    num_rows, rows_stride, grad_stride = None, 0, 0
-    for t, name in ((rows, "rows"), (grad_rows, "grad_rows")):
-        if t is None:
-            continue
-        count, width, stride = _matrix(t, name)
-        _refuse_unless(width == dim and t.dtype == grad_out.dtype,
-                       "rows, grad_rows and grad_out differ in dim or type")
+    count = num_rows = None
+    rows_stride = rows_at = grad_stride = grad_at = 0
+    if rows is not None:
+        num_rows, _, rows_stride, rows_at = _matrix(rows, "rows", 0, index, dim, dtype)
+    if grad_rows is not None:
+        count, _, grad_stride, grad_at = _matrix(grad_rows, "grad_rows", 0, index, dim, dtype)
         _refuse_unless(num_rows in (None, count), "rows and grad_rows differ in rows")
         num_rows = count
-        if t is rows:
-            rows_stride = stride
-        if t is grad_rows:
-            grad_stride = stride
     if positions is not None:
-        p, slots = _positions(n, positions)
+        p, slots = _positions(positions, n, index)
     else:
         p, slots = None, _by_place(slots, weights, grad_weights)
+    w = gw = None
     w_kind = 0
-    for t, name in ((weights, "weights"), (grad_weights, "grad_weights")):
-        if t is not None:
-            w_kind = _weights(t, name, n, slots, kind)
-    if weights is not None and grad_weights is not None:
-        _refuse_unless(weights.dtype == grad_weights.dtype,
+    if weights is not None:
+        w, w_kind = _weights(weights, "weights", n, index, slots, kind)
+    if grad_weights is not None:
+        _refuse_unless(weights is None or weights.dtype == grad_weights.dtype,
                        "weights and grad_weights differ in type")
-    index = _one_device(grad_out, rows, grad_rows, positions, weights, grad_weights)
-    _call_on(index, stream, lib().hkv_combine_rows_backward, n, slots, dim, kind, _ptr(rows),
-             rows_stride, num_rows, p, _ptr(weights), w_kind, grad_out.data_ptr(), out_stride,
-             _ptr(grad_rows), grad_stride, _ptr(grad_weights))
+        gw, w_kind = _weights(grad_weights, "grad_weights", n, index, slots, kind)
+    _call_on(index, stream, lib().hkv_combine_rows_backward, n, slots, dim, kind, rows_at,
+             rows_stride, num_rows, p, w, w_kind, out_at, out_stride, grad_at, grad_stride, gw)
 
 
 class PagePool:
@@ -1078,7 +1066,7 @@ class PagePool:
             _refuse_unless(t.is_contiguous(), f"plane {k} must be contiguous")
             _refuse_unless(t.numel() > 0, f"plane {k} is empty")
         if table is not None:
-            rows, width, stride = _matrix(table, "table")
+            rows, width, stride, _ = _matrix(table, "table", 0, table.get_device())
             _refuse_unless(table.dtype == torch.int32, "table must be int32")
             _refuse_unless(num_rows in (None, rows) and max_pages in (None, width),
                            "table differs from num_rows or max_pages")
@@ -1089,9 +1077,9 @@ class PagePool:
                         ("num_rows", num_rows), ("max_pages", max_pages)):
             _refuse_unless(0 < v < 1 << 31, f"{name} must be positive and below 2^31")
         if refs is not None:
-            _list(refs, "refs", num_pages, torch.int32)
+            _list(refs, "refs", num_pages, refs.get_device(), torch.int32)
         if lengths is not None:
-            _list(lengths, "lengths", num_rows, torch.int32)
+            _list(lengths, "lengths", num_rows, lengths.get_device(), torch.int32)
         _refuse_unless(device.type == "cuda", "the tensors must be on a CUDA device")
         for t in given:
             _refuse_unless(t.device == device, "the tensors are on different devices")
@@ -1138,10 +1126,7 @@ class PagePool:
     def _numbers(self, t, name, n, dtype=None):
         if n < 0:
             raise HkvException("n must not be negative")
-        address = _list(t, name, n, dtype or _TORCH.int32)
-        if t.get_device() != self._index:
-            raise HkvException(f"{name} is not on the pool's device")
-        return address
+        return _list(t, name, n, self._index, dtype or _TORCH.int32)
 
     def copy(self, n, src, dst, stream=None):
         """Copies page src[i] to page dst[i] in every plane. A destination may
@@ -1193,7 +1178,7 @@ class PagePool:
         if table_out is not None:
             _refuse_unless(table_out.dtype == torch.int32 and table_out.shape == self.table.shape
                            and table_out.device == self.device, "table_out is not like table")
-            _refuse_unless(_matrix(table_out, "table_out")[2] == self._table_stride,
+            _refuse_unless(_matrix(table_out, "table_out", 0, self._index)[2] == self._table_stride,
                            "table_out and table differ in stride")
             t = table_out.data_ptr()
         _check(lib().hkv_pages_compact(self._h, m, t, r, self._on_stream(stream)))
