@@ -41,6 +41,18 @@ void launch(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem,
   }
 }
 
+// Leave for a launch with `smem` bytes of dynamic shared memory. 48 KB need none,
+// but hold a kernel's own arrays too (272 bytes at most here): asked for from 46 KB
+// on.
+constexpr size_t kMostShared = 220 * 1024;
+
+template <class K>
+void allow_shared(K kernel, size_t smem) {
+  if (smem > 46 * 1024)
+    CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>(smem)));
+}
+
 __device__ __forceinline__ void after_previous() {
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();  // the next one may be set up

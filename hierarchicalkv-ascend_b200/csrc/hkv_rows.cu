@@ -376,7 +376,7 @@ SortPlan sort_plan(size_t n, uint32_t num_groups) {
     if (p.blocks == 1)
       p.threads = std::max(128u, std::min(kClusterThreads, ((m + p.items - 1) / p.items + 63) / 64 * 64));
     p.smem = cluster_smem(num_groups, p.threads, p.items);
-    p.cluster = p.smem <= 220 * 1024;
+    p.cluster = p.smem <= kMostShared;
   }
   if (p.cluster) {
     p.workspace = 16;
@@ -414,13 +414,6 @@ void with_items(uint32_t items, F f) {
   }
 }
 
-template <class K>
-void allow_smem(K kernel, size_t smem) {
-  if (smem > 48 * 1024)
-    CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(smem)));
-}
-
 template <class Id>
 void launch_sort(size_t n, const void* groups, uint32_t num_groups, int32_t* offsets,
                  int32_t* positions, int32_t* order, void* workspace, cudaStream_t s) {
@@ -431,7 +424,7 @@ void launch_sort(size_t n, const void* groups, uint32_t num_groups, int32_t* off
     if (p.cluster) {
       if constexpr (kItems <= static_cast<int>(kClusterItems)) {
         auto kernel = group_cluster_kernel<Id, kItems, kBits>;
-        allow_smem(kernel, p.smem);
+        allow_shared(kernel, p.smem);
         launch(kernel, p.blocks, p.threads, p.smem, s, p.blocks, count, groups,
                num_groups, p.blocks, offsets, positions, order);
       }
@@ -448,7 +441,7 @@ void launch_sort(size_t n, const void* groups, uint32_t num_groups, int32_t* off
       launch(group_scan_kernel, (num_groups + 7) / 8, 256, 0, s, 1, num_groups, p.blocks, counts,
              totals);
     auto kernel = group_place_kernel<Id, kItems, kBits>;
-    allow_smem(kernel, p.smem);
+    allow_shared(kernel, p.smem);
     launch(kernel, p.blocks, kSortThreads, p.smem, s, 1, count, groups, num_groups, p.run,
            static_cast<const uint32_t*>(counts), static_cast<const uint32_t*>(totals), offsets,
            positions, order);

@@ -1,0 +1,43 @@
+"""Calls that are the first of their process, at sizes where a block's shared memory
+ends at the 48 KB that need no leave: the arrays that a kernel declares count
+too. What a process ran before may raise a kernel's limit, so each case has its own.
+Results are whole numbers and equal the definition's."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+import hkv_b200 as H
+
+pytestmark = pytest.mark.gpu
+
+START = f"""
+import sys
+sys.path.insert(0, {os.path.dirname(os.path.abspath(H.__file__))!r})
+import torch
+import hkv_b200 as H
+def i32(*shape): return torch.zeros(shape, dtype=torch.int32, device="cuda")
+"""
+
+SORT = """
+n, groups = {n}, {groups}
+ids = torch.randint(0, groups, (n,), generator=torch.Generator().manual_seed(n))
+offsets, positions, order = i32(groups + 1), i32(n), i32(n)
+H.group_tokens(n, ids.cuda(), groups, offsets, positions, order)
+want = torch.sort(ids, stable=True).indices
+assert torch.equal(order.cpu().long(), want)
+assert torch.equal(positions.cpu().long()[want], torch.arange(n))
+assert torch.equal(offsets.cpu().long()[1:], torch.bincount(ids, minlength=groups).cumsum(0))
+"""
+
+def first_call(code):
+    done = subprocess.run([sys.executable, "-c", START + code], capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("n,groups", [(512, 1024), (960, 576), (8192, 428), (20000, 214),
+                                      (40000, 1168)])
+def test_group_tokens(n, groups):
+    first_call(SORT.format(n=n, groups=groups))
