@@ -43,14 +43,17 @@ void launch(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem,
 
 // Leave for a launch with `smem` bytes of dynamic shared memory. 48 KB need none,
 // but hold a kernel's own arrays too (272 bytes at most here): asked for from 46 KB
-// on.
+// on. The limit belongs to the kernel on the device, not to the launch, and other
+// host threads launch the same kernel: it is always set to the one value that
+// covers every launch (227 KB is the most a block can have), so that no call
+// takes away what another one needs.
 constexpr size_t kMostShared = 220 * 1024;
 
 template <class K>
 void allow_shared(K kernel, size_t smem) {
   if (smem > 46 * 1024)
     CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  static_cast<int>(smem)));
+                                  static_cast<int>(kMostShared)));
 }
 
 __device__ __forceinline__ void after_previous() {

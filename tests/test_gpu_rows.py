@@ -11,6 +11,8 @@ the relative bound ends.
 * grad_weights: dim products and additions in any order, dim u sum |g y|, then
   one rounding.
 """
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -140,6 +142,38 @@ def test_group_tokens_on_two_streams_at_once():
         want = sorted_reference(ids[k], groups)
         assert np.array_equal(out[k][1].cpu().numpy(), want[1])
         assert np.array_equal(out[k][2].cpu().numpy(), want[2])
+
+
+@pytest.mark.parametrize("n,first,second", [(30000, 300, 400), (40000, 1500, 4000)])
+def test_group_tokens_from_host_threads(n, first, second):
+    """Host threads, each with a stream and a workspace, launch the same kernels with
+    more than 48 KB of shared memory, of two sizes. The library's calls are made
+    one right after the other, so that they meet."""
+    calls, work = 3000, []
+    for groups in (first, second) * 2:
+        ids = torch.randint(0, groups, (n,), generator=seeded(groups), device="cuda")
+        scratch = torch.zeros(H.group_workspace(n, groups), dtype=torch.uint8, device="cuda")
+        work.append((ids, groups, (i32(groups + 1), i32(n), i32(n)), scratch, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    ready, statuses = threading.Barrier(len(work), timeout=60), []
+
+    def sort(ids, groups, out, scratch, stream):
+        call = H.lib().hkv_group_tokens
+        args = (n, ids.data_ptr(), 1, groups, *(t.data_ptr() for t in out), scratch.data_ptr(),
+                scratch.numel(), stream.cuda_stream)
+        ready.wait()
+        statuses.extend([call(*args) for _ in range(calls)])
+
+    threads = [threading.Thread(target=sort, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(statuses) == calls * len(work) and not any(statuses)
+    for ids, groups, out, _, _ in work:
+        want = sorted_reference(ids, groups)
+        assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip(out, want))
 
 
 # ---- dispatch_rows -----------------------------------------------------------
