@@ -747,12 +747,9 @@ class PagesImpl {
       if (fork_smem(o.num_rows, o.num_rows) > 48 * 1024)
         CUDA_TRY(cudaFuncSetAttribute(fork_columns_kernel,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
-      if (o.num_rows * 4ull > 48 * 1024)
-        with_width([&](auto width) {
-          CUDA_TRY(cudaFuncSetAttribute(resize_plan_kernel<decltype(width)::value>,
-                                        cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        kMostShared));
-        });
+      with_width([&](auto width) {
+        allow_shared(resize_plan_kernel<decltype(width)::value>, o.num_rows * 4ull);
+      });
     } catch (...) {
       mem_.free_device(scratch_);
       throw;

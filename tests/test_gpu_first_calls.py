@@ -31,6 +31,16 @@ assert torch.equal(positions.cpu().long()[want], torch.arange(n))
 assert torch.equal(offsets.cpu().long()[1:], torch.bincount(ids, minlength=groups).cumsum(0))
 """
 
+RESIZE = """
+rows = {rows}
+pool = H.PagePool([torch.zeros((2 * rows, {width}), dtype=torch.uint8, device="cuda")], 4, rows, 2)
+every = torch.arange(rows, device="cuda", dtype=torch.int32)
+status = torch.zeros(rows, dtype=torch.bool, device="cuda")
+pool.resize(rows, every, torch.full_like(every, 5), status)
+assert status.all() and (pool.refs == 1).all() and (pool.lengths == 5).all()
+assert torch.equal(pool.table.view(-1), torch.arange(2 * rows, device="cuda", dtype=torch.int32))
+"""
+
 def first_call(code):
     done = subprocess.run([sys.executable, "-c", START + code], capture_output=True, text=True,
                           timeout=300)
@@ -41,3 +51,8 @@ def first_call(code):
                                       (40000, 1168)])
 def test_group_tokens(n, groups):
     first_call(SORT.format(n=n, groups=groups))
+
+
+@pytest.mark.parametrize("rows,width", [(12288, 16), (12221, 5)])
+def test_resize(rows, width):
+    first_call(RESIZE.format(rows=rows, width=width))
