@@ -744,9 +744,7 @@ class PagesImpl {
       CUDA_TRY(cudaMemset(arrived_, 0, 4));
       CUDA_TRY(cudaDeviceSynchronize());
       // kernels that this pool may give more than 48 KB of shared memory
-      if (fork_smem(o.num_rows, o.num_rows) > 48 * 1024)
-        CUDA_TRY(cudaFuncSetAttribute(fork_columns_kernel,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+      allow_shared(fork_columns_kernel, fork_smem(o.num_rows, o.num_rows));
       with_width([&](auto width) {
         allow_shared(resize_plan_kernel<decltype(width)::value>, o.num_rows * 4ull);
       });

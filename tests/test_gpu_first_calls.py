@@ -41,6 +41,19 @@ assert status.all() and (pool.refs == 1).all() and (pool.lengths == 5).all()
 assert torch.equal(pool.table.view(-1), torch.arange(2 * rows, device="cuda", dtype=torch.int32))
 """
 
+FORK = """
+rows = {rows}
+pool = H.PagePool([], 4, rows, 17, num_pages=17 * rows)
+every = torch.arange(rows, device="cuda", dtype=torch.int32)
+pool.resize(rows, every, every % 69)
+lengths, table = pool.lengths.clone(), pool.table.clone()
+pool.fork(rows, every, every.flip(0).contiguous())
+assert torch.equal(pool.lengths, lengths.flip(0))
+held = torch.arange(17, device="cuda")[None] < ((pool.lengths + 3) // 4)[:, None]
+assert torch.equal(pool.table[held], table.flip(0)[held])
+"""
+
+
 def first_call(code):
     done = subprocess.run([sys.executable, "-c", START + code], capture_output=True, text=True,
                           timeout=300)
@@ -56,3 +69,7 @@ def test_group_tokens(n, groups):
 @pytest.mark.parametrize("rows,width", [(12288, 16), (12221, 5)])
 def test_resize(rows, width):
     first_call(RESIZE.format(rows=rows, width=width))
+
+
+def test_fork():
+    first_call(FORK.format(rows=945))
