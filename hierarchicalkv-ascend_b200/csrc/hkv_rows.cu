@@ -394,6 +394,13 @@ SortPlan sort_plan(size_t n, uint32_t num_groups) {
   return p;
 }
 
+// Scratch that serves every sort of n places or fewer. What one sort needs rises
+// and falls: the blocks halve where the tiles of a block, or their places, double.
+size_t sort_workspace(size_t n, uint32_t num_groups) {
+  const size_t blocks = std::min<size_t>(kSortBlocks, (n + kSortThreads - 1) / kSortThreads);
+  return std::max<size_t>(16, (blocks + 1) * num_groups * 4);
+}
+
 // calls f with kItems and kBits as constants
 template <class F>
 void with_bits(uint32_t num_groups, F f) {
@@ -886,7 +893,7 @@ int hkv_group_workspace(size_t n, uint32_t num_groups, size_t* out_bytes) {
   HKV_REQUIRE(n <= hkvb::kMaxCount, HKV_ERR_INVALID, "n must be below 2^31");
   HKV_REQUIRE(num_groups > 0 && num_groups <= HKV_MAX_GROUPS, HKV_ERR_INVALID,
               "num_groups must be 1 to 4096");
-  *out_bytes = hkvb::sort_plan(n, num_groups).workspace;
+  *out_bytes = hkvb::sort_workspace(n, num_groups);
   HKV_API_END
 }
 

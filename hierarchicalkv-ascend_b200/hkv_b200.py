@@ -915,7 +915,8 @@ def _call_on(index, stream, fn, n, *args):
 
 
 def group_workspace(n: int, num_groups: int) -> int:
-    """Bytes of scratch that group_tokens needs for n places."""
+    """Bytes of scratch that group_tokens needs for n places or fewer, and
+    num_groups groups or fewer."""
     _refuse_unless(n >= 0 and num_groups >= 0, "n and num_groups must not be negative")
     _refuse_unless(num_groups < 1 << 32, "num_groups must be 1 to 4096")
     out = _SZ(0)

@@ -490,7 +490,8 @@ typedef enum { HKV_ID_I32 = 0, HKV_ID_I64 = 1 } hkv_id_type;
 /* Most groups of one hkv_group_tokens call. */
 #define HKV_MAX_GROUPS 4096
 
-/* Bytes of scratch that hkv_group_tokens needs for n places. */
+/* Bytes of scratch that hkv_group_tokens needs for n places or fewer, and for
+ * num_groups groups or fewer: scratch for the largest call serves all. */
 int hkv_group_workspace(size_t n, uint32_t num_groups, size_t* out_bytes);
 
 /* Stable sort of n places by groups[i] (id_type): positions[i] is the row of

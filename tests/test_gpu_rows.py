@@ -144,6 +144,16 @@ def test_group_tokens_on_two_streams_at_once():
         assert np.array_equal(out[k][2].cpu().numpy(), want[2])
 
 
+@pytest.mark.parametrize("groups", [64, 3000])
+def test_scratch_of_the_largest_batch(groups):
+    """Scratch sized once serves every smaller call."""
+    largest = 200000
+    scratch = torch.zeros(H.group_workspace(largest, groups), dtype=torch.uint8, device="cuda")
+    for n in (0, 1, 1000, 1024, 1025, 32768, 32769, 150000, 151552, 151553, largest):
+        ids = torch.randint(-1, groups, (n,), generator=seeded(n), device="cuda")
+        check_sort(ids, groups, workspace=scratch)
+
+
 @pytest.mark.parametrize("n,first,second", [(30000, 300, 400), (40000, 1500, 4000)])
 def test_group_tokens_from_host_threads(n, first, second):
     """Host threads, each with a stream and a workspace, launch the same kernels with

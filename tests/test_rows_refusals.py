@@ -32,6 +32,18 @@ def test_group_workspace_refuses(n, groups):
         H.group_workspace(n, groups)
 
 
+@pytest.mark.parametrize("groups", [1, 8, 64, 428, 1168, 3000, 4096])
+def test_group_workspace_never_falls(groups):
+    """Scratch for n places serves every call with fewer. The borders of the forms
+    and of the tiles' sizes lie at multiples of 512."""
+    borders = sorted({max(0, k * step + d) for step in (512, 4096, 75776, 303104)
+                      for k in range(0, 40) for d in (-1, 0, 1)} | {1 << 24, (1 << 31) - 1})
+    sizes = [H.group_workspace(n, groups) for n in borders]
+    assert all(a <= b for a, b in zip(sizes, sizes[1:]))
+    # nor with more groups
+    assert all(H.group_workspace(n, groups) <= H.group_workspace(n, 4096) for n in borders)
+
+
 GROUP = dict(n=4, groups=SOME, id_type=0, num_groups=8, offsets=SOME, positions=SOME, order=SOME,
              workspace=SOME, workspace_bytes=1 << 20, stream=None)
 
