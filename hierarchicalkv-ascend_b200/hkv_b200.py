@@ -914,11 +914,17 @@ def _call_on(index, stream, fn, n, *args):
         _check(status)
 
 
+def _check_groups(num_groups):
+    """Here, as the C ABI would see its low 32 bits alone."""
+    if not 0 < num_groups <= 4096:
+        raise HkvException("num_groups must be 1 to 4096")
+
+
 def group_workspace(n: int, num_groups: int) -> int:
     """Bytes of scratch that group_tokens needs for n places or fewer, and
     num_groups groups or fewer."""
-    _refuse_unless(n >= 0 and num_groups >= 0, "n and num_groups must not be negative")
-    _refuse_unless(num_groups < 1 << 32, "num_groups must be 1 to 4096")
+    _refuse_unless(n >= 0, "n must not be negative")
+    _check_groups(num_groups)
     out = _SZ(0)
     _check(lib().hkv_group_workspace(n, num_groups, ctypes.byref(out)))
     return out.value
@@ -934,6 +940,7 @@ def group_tokens(n, groups, num_groups, offsets, positions, order=None, workspac
     uint8 tensor of group_workspace(n, num_groups) bytes, allocated here when
     None; calls that may overlap need their own."""
     torch = _torch()
+    _check_groups(num_groups)
     ids, index = torch.ids.get(groups.dtype), groups.get_device()
     if ids is None:
         raise HkvException(f"groups must be int32 or int64, not {groups.dtype}")

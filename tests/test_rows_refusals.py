@@ -44,6 +44,16 @@ def test_group_workspace_never_falls(groups):
     assert all(H.group_workspace(n, groups) <= H.group_workspace(n, 4096) for n in borders)
 
 
+@pytest.mark.parametrize("groups", [8 - (1 << 32), 8 + (1 << 32), -1, 0, 4097])
+@pytest.mark.parametrize("scratch", [None, 1 << 16])
+def test_group_tokens_refuses_numbers_of_groups(groups, scratch):
+    """Before offsets, which are num_groups + 1, are looked at."""
+    work = None if scratch is None else torch.zeros(scratch, dtype=torch.uint8)
+    offsets = i32(max(groups + 1, 1) if groups < 1 << 20 else 16)
+    with pytest.raises(H.HkvException, match="num_groups must be 1 to 4096"):
+        H.group_tokens(8, i32(8), groups, offsets, i32(8), workspace=work)
+
+
 GROUP = dict(n=4, groups=SOME, id_type=0, num_groups=8, offsets=SOME, positions=SOME, order=SOME,
              workspace=SOME, workspace_bytes=1 << 20, stream=None)
 
