@@ -885,6 +885,7 @@ def _by_place(slots, *shaped):
             slots = t.shape[-1]
     _refuse_unless(slots is not None and slots > 0,
                    "without positions and weights, slots must be given")
+    _refuse_unless(slots < 1 << 31, "slots must be below 2^31")
     return slots
 
 
@@ -923,7 +924,7 @@ def _check_groups(num_groups):
 def group_workspace(n: int, num_groups: int) -> int:
     """Bytes of scratch that group_tokens needs for n places or fewer, and
     num_groups groups or fewer."""
-    _refuse_unless(n >= 0, "n must not be negative")
+    _refuse_unless(0 <= n < 1 << 31, "n must not be negative, and below 2^31")
     _check_groups(num_groups)
     out = _SZ(0)
     _check(lib().hkv_group_workspace(n, num_groups, ctypes.byref(out)))

@@ -54,6 +54,18 @@ def test_group_tokens_refuses_numbers_of_groups(groups, scratch):
         H.group_tokens(8, i32(8), groups, offsets, i32(8), workspace=work)
 
 
+def test_slots_beyond_32_bits():
+    rows, x = torch.zeros(8, 8), torch.zeros(4, 8)
+    for slots in (1 << 31, (1 << 32) + 2, (1 << 64) + 2):
+        with pytest.raises(H.HkvException, match="slots"):
+            H.combine_rows(4, rows, None, None, x, slots=slots)
+        with pytest.raises(H.HkvException, match="slots"):
+            H.combine_rows_backward(4, None, None, None, x, rows, slots=slots)
+    for n in (1 << 31, (1 << 64) + 5):
+        with pytest.raises(H.HkvException):
+            H.group_workspace(n, 8)
+
+
 GROUP = dict(n=4, groups=SOME, id_type=0, num_groups=8, offsets=SOME, positions=SOME, order=SOME,
              workspace=SOME, workspace_bytes=1 << 20, stream=None)
 
