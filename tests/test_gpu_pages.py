@@ -324,6 +324,43 @@ def test_many_rows(rows):
     b.fork([1, 2], [2, 1])
 
 
+def test_time_of_a_fork_grows_with_its_list():
+    """No faster than the list: 32 times the entries take 64 times as long at most,
+    where comparing every entry with every other would take a thousand times."""
+    rows = 1 << 18
+    pool = H.PagePool([], 4, rows, 1, num_pages=8)
+    order = torch.randperm(rows, device="cuda").to(torch.int32)
+
+    def milliseconds(n):
+        times = []
+        for _ in range(7):
+            begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            begin.record()
+            pool.fork(n, order, order)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        return sorted(times)[3]
+
+    milliseconds(rows)
+    assert milliseconds(rows) <= 64 * milliseconds(rows >> 5)
+
+
+def test_long_lists_of_long_rows():
+    """Thousands of entries, rows of more than one block's columns, destinations named
+    several times and numbers that no row has; forked again and again."""
+    rng = np.random.default_rng(11)
+    rows, width = 2500, 1100
+    b = Both(30000, 4, rows, width, ())
+    some = rng.permutation(rows)[:40].tolist()
+    b.resize(some, rng.integers(0, 4 * width + 1, 20).tolist() + rng.integers(0, 9, 20).tolist())
+    for low, high in ((0, rows), (-2, rows + 2), (0, 30)):
+        dst = rng.integers(low, high, rows).tolist()
+        dst[-1] = dst[0]
+        b.fork(rng.integers(-1, rows + 1, rows).tolist(), dst)
+        b.fork(rng.permutation(rows).tolist(), rng.permutation(rows).tolist())
+
+
 def test_pages_of_several_chunks_and_many_entries():
     """Page copies that a few blocks of an entry take in steps."""
     b = Both(2700, 4, 1300, 2, (33000, 16), 4)
