@@ -550,3 +550,39 @@ def test_prefix_index_of_a_cache():
         if f[k]:
             assert plane[got_all[k], 0] == first[k]
     index.close()
+
+
+def test_prefix_index_that_loses_half_of_its_blocks():
+    """Six of twelve blocks evicted: their pages are let go, the others are found and
+    hold what they held, before and after a compaction."""
+    size, pages = 4, 64
+    plane = torch.arange(pages, device="cuda", dtype=torch.int32)[:, None].repeat(1, 8)
+    pool = H.PagePool([plane], size, 2, 16)
+    index = H.HashTable(H.EvictStrategy.kLru, value_dtype="uint32")
+    index.init(H.HashTableOptions(init_capacity=128, max_capacity=128,
+                                  max_hbm_for_vectors=1 << 20, dim=1))
+    hashes = torch.arange(1, 13, device="cuda", dtype=torch.int64) * 7919
+    pool.resize(2, i32([0, 1]), i32([5 * size, 12 * size]))
+    pool.free(1, i32([0]))
+    first = pool.table[1, :12].contiguous()
+    assert first.tolist() == list(range(5, 17))
+    index.insert_or_assign(12, hashes, first)
+    pool.hold(12, first)
+    pool.free(1, i32([1]))
+    n = 128 - 12 + 6
+    more = torch.arange(1000, 1000 + n, device="cuda", dtype=torch.int64) * 104729
+    gone, lost = torch.zeros(n, dtype=torch.int64, device="cuda"), i32([-1] * n)
+    count = index.insert_and_evict(n, more, i32([-1] * n), None, gone, lost)
+    assert count == 6 and all(5 <= p < 17 for p in lost[:6].tolist())
+    pool.hold(count, lost, -1)
+    found, got = torch.zeros(12, dtype=torch.bool, device="cuda"), i32([-1] * 12)
+    index.find(12, hashes, got, found)
+    kept = [k for k in range(12) if found[k]]
+    assert len(kept) == 6
+    assert [got[k].item() for k in kept] == [first[k].item() for k in kept]
+    assert sorted(first[k].item() for k in kept) == pool.refs.nonzero()[:, 0].tolist()
+    page_map = i32([0] * pages)
+    pool.compact(page_map)
+    assert pool.refs.tolist() == [1] * 6 + [0] * (pages - 6)
+    assert [plane[page_map[first[k]], 0].item() for k in kept] == [first[k].item() for k in kept]
+    index.close()

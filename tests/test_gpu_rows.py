@@ -408,6 +408,31 @@ def test_offsets_over_32_bits():
     assert (rows16[-1] == 1).all() and (rows16[0] == 1).all() and not rows16[1].any()
 
 
+def test_more_words_than_32_bits_number():
+    """Rows of an odd number of 2-byte elements, 2^31 of them and some more, which
+    take more than one launch: all rows there and back, by position and by place."""
+    dim = 4097
+    n = (1 << 31) // dim + 50
+    x = torch.randint(-128, 128, (n, dim), generator=seeded(1), device="cuda", dtype=torch.int8)
+    x = x.to(BF16)
+    at = torch.arange(n - 1, -1, -1, device="cuda", dtype=torch.int32).view(n, 1)
+    at[5] = at[n - 5] = -1
+    rows = torch.zeros((n, dim), dtype=BF16, device="cuda")
+    H.dispatch_rows(n, x, at, rows)
+    x[5], x[n - 5] = 0, 0
+    assert torch.equal(rows.flip(0), x)
+    out = torch.full((n, dim), 7.0, dtype=BF16, device="cuda")
+    H.combine_rows(n, rows, at, None, out)
+    assert torch.equal(out, x)
+    del rows, at
+    two = torch.stack([x, x], 1).view(2 * n, dim)
+    two = two[:2 * n - 1]  # the last place has no row
+    out.fill_(7.0)
+    H.combine_rows(n, two, None, None, out, slots=2)
+    x[:n - 1] *= 2
+    assert torch.equal(out, x)
+
+
 def test_captured_and_replayed():
     """The whole way there and back in a graph, replayed on other inputs."""
     n, slots, groups, dim = 96, 4, 16, 64
