@@ -57,9 +57,9 @@ __device__ __forceinline__ int load_group(const void* groups, uint32_t i, uint32
 }
 
 // Lanes of the warp with the same id, by one ballot per bit of an id; of no
-// meaning for a lane without one. (With __match_any_sync 131072 places of 128
-// groups took 22 us in one launch, 18 so; a million in three launches 22.6 with
-// a loop over the bits, 21.6 with kBits of them.)
+// meaning for a lane without one. (us a sort, with __match_any_sync, with twelve
+// ballots for any number of groups, and so: 32768 places of 128 groups 9.6, 8.6,
+// 7.7; a million of 8 groups 13.0, 18.6, 12.5, of 64 groups 25.4, 21.0, 18.5.)
 template <int kBits>
 __device__ __forceinline__ uint32_t same_id(int id) {
   uint32_t same = __ballot_sync(~0u, id >= 0);
@@ -105,8 +105,8 @@ __device__ __forceinline__ uint32_t scan_over_warps(uint16_t* cnt, uint32_t warp
 // One launch: `blocks` blocks of one cluster, block b takes the places from
 // b * blockDim.x * kItems. The rows of order are written from shared memory
 // in the block's sorted order, so that a group's run is written in whole
-// sectors. Bound by the latency of its phases: 128 places of 64 groups 1.8 us,
-// 4096 4.6, 32768 7.0 (back to back in a graph).
+// sectors. Bound by the latency of its phases: 128 places of 64 groups 2.1 us,
+// 4096 5.1, 32768 7.5 (back to back in a graph).
 constexpr uint32_t kClusterThreads = 1024;
 
 template <class Id, int kItems, int kBits>
@@ -186,8 +186,8 @@ __global__ void __launch_bounds__(kClusterThreads)
 }
 
 // Three launches (two where the counts are few). Blocks take runs of tiles;
-// counts[g * blocks + b]. 131072 places of 64 groups take 7.2 us, a million 18.0,
-// of 8 groups 12.0.
+// counts[g * blocks + b]. 131072 places of 64 groups take 7.5 us, a million 18.5,
+// of 8 groups 12.5.
 
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
@@ -246,8 +246,8 @@ __global__ void group_scan_kernel(uint32_t num_groups, uint32_t blocks, uint32_t
 }
 
 // What bounds it is the latency of the chain within a warp, not memory: four
-// blocks per SM (32 registers) take a million places of 8 groups in 12.2 us for
-// all launches, two in 13.4; the ballots of a warp's places come first, together.
+// blocks per SM (32 registers) take a million places of 8 groups in 12.5 us for
+// all launches, two in 13.7; the ballots of a warp's places come first, together.
 template <class Id, int kItems, int kBits>
 __global__ void __launch_bounds__(kSortThreads, 4)
     group_place_kernel(uint32_t n, const void* groups, uint32_t num_groups,
@@ -356,10 +356,10 @@ size_t cluster_smem(uint32_t num_groups, uint32_t threads, uint32_t items) {
 }
 
 // Places of the one-launch form: 8 blocks of 1024 threads, four places each.
-// Measured (us a sort in a graph, 64 groups, one launch against three): 128
-// places 2.0 / 5.1, 4096 5.0 / 5.3, 16384 5.4 / 5.9, 32768 7.3 / 5.9, 131072
-// 16.6 / 7.2. The two further launches cost 4 us of host time where the host
-// is what a pass waits for, so the border is above the crossing.
+// Measured (us a sort in a graph, 64 groups, one launch against the long form):
+// 128 places 2.1 / 5.2, 4096 5.1 / 6.2, 16384 5.5 / 5.8, 32768 7.5 / 7.0. The
+// further launches cost 4 us of host time where the host is what a pass waits
+// for, so the border is above the crossing; a graph loses 0.5 us of 32768 places.
 constexpr uint32_t kMaxCluster = 8;
 constexpr uint32_t kClusterItems = 4;
 
@@ -641,8 +641,9 @@ __global__ void __launch_bounds__(kRowThreads, 6)
 // kTeam threads per token hold a pack of its gradient at a time and go over its
 // slots, kAhead rows in flight: the rows' gradients, and the inner products in
 // per-thread sums joined by a fixed tree of shuffles (and, for teams of several
-// warps, through shared memory). A token's gradient is read once, its rows once:
-// bound by memory, 8192 tokens of 8 KB with eight rows each, 1131 MB, in 176 us
+// warps, through shared memory). A token's rows are read once, its gradient once
+// for every kAhead slots, from a cache after the first time: bound by memory, 8192
+// tokens of 8 KB with eight rows each, 1131 MB, in 176 us
 // (6.4 TB/s). A warp per place, which reads the token's gradient for each of its
 // slots, took 195 us, and 379 with four packs in flight.
 template <class T, int kVec, int kTeam>
@@ -772,7 +773,9 @@ uint64_t stride_or(size_t stride, size_t dim, const char* what) {
 }
 
 // largest word (16 bytes at most) that addresses, strides and rows are
-// multiples of
+// multiples of. A row of an odd number of elements moves by single elements, which
+// leaves too few bytes in flight: dispatch of 18071 rows of 2033 bf16 to six places
+// takes 168 us where its bytes take 77 at the copy bandwidth.
 uint32_t word_bytes(std::initializer_list<const void*> ptrs, std::initializer_list<uint64_t> sizes) {
   uint64_t all = 16;
   for (const void* p : ptrs) all |= reinterpret_cast<uintptr_t>(p);
