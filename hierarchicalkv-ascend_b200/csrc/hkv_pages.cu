@@ -765,6 +765,9 @@ class PagesImpl {
     staged_ = reinterpret_cast<int32_t*>(scratch_ + a_staged);
     if (long_forks) last_of_ = reinterpret_cast<int32_t*>(scratch_ + a_last_of);
     try {
+      // (memory of an allocator that goes by streams may still be written by work
+      // that is not done: its order is another stream's)
+      CUDA_TRY(cudaDeviceSynchronize());
       CUDA_TRY(cudaMemset(arrived_, 0, 4));
       if (long_forks) CUDA_TRY(cudaMemset(last_of_, 0xff, o.num_rows * 4ull));
       CUDA_TRY(cudaDeviceSynchronize());

@@ -480,6 +480,32 @@ def test_scratch_from_a_given_allocator():
     assert not made.blocks
 
 
+def test_scratch_that_pending_work_still_writes():
+    """A pool made on a side stream gets memory that a kernel before it, not yet run,
+    writes: in the order of that stream this comes first."""
+    def state():
+        return dict(refs=i32([0] * 40), table=i32([[-1] * 8] * 3000), lengths=i32([0] * 3000))
+
+    first = H.TorchAllocator()
+    like = H.PagePool([], 4, allocator=first, **state())
+    (size,) = [block.numel() for block in first.blocks.values()]
+    like.close()
+    given, side, made = state(), torch.cuda.Stream(), H.TorchAllocator()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        pending = torch.empty(size, dtype=torch.uint8, device="cuda")
+        address = pending.data_ptr()
+        torch.cuda._sleep(100_000_000)
+        pending.fill_(3)
+        del pending
+        pool = H.PagePool([], 4, allocator=made, **given)
+    assert list(made.blocks) == [address]
+    for n in (3, 3000):  # both forms of a fork
+        given["lengths"][:2] = i32([9, 32])
+        pool.fork(n, i32([0, 1] + [1] * (n - 2)), i32([1, 0] + list(range(2, n))))
+        assert pool.lengths[:n].tolist() == [32, 9] + [32] * (n - 2)
+
+
 def test_failing_allocator():
     class Nothing:
         def alloc(self, memory_type, size, flags):
