@@ -361,6 +361,22 @@ def test_long_lists_of_long_rows():
         b.fork(rng.permutation(rows).tolist(), rng.permutation(rows).tolist())
 
 
+def test_long_list_captured_and_replayed():
+    rng = np.random.default_rng(12)
+    rows = 2600
+    b = Both(9000, 4, rows, 3, (), 12)
+    b.resize(list(range(rows)), rng.integers(0, 13, rows).tolist())
+    src, dst = i32(rng.permutation(rows).tolist()), i32([0] * rows)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.pool.fork(rows, src, dst)
+    for low, high in ((0, rows), (0, 9), (-3, rows)):
+        dst.copy_(i32(rng.integers(low, high, rows).tolist()))
+        graph.replay()
+        b.model.fork(src.tolist(), dst.tolist())
+        b.check()
+
+
 def test_pages_of_several_chunks_and_many_entries():
     """Page copies that a few blocks of an entry take in steps."""
     b = Both(2700, 4, 1300, 2, (33000, 16), 4)
