@@ -667,7 +667,7 @@ class OnDevice {
 }  // namespace
 
 class PagesImpl {
-  static constexpr int kMostShared = 200 * 1024;
+  static constexpr size_t kMostPlanned = 200 * 1024;  // shared memory of a plan or fork
   static constexpr uint32_t kOneLaunchShares = 256, kOneLaunchMoves = 1024;
   static constexpr uint32_t kPageStep = 1024;  // pages of a row that one share goes over
   static constexpr uint32_t kForkSearched = 2048;  // entries of a list that its blocks search
@@ -742,11 +742,11 @@ class PagesImpl {
     const size_t a_forks = part(o.num_rows * sizeof(Fork));
     const size_t a_wants = part(o.num_rows * sizeof(Want));
     const size_t a_needs = part(o.num_rows * 4ull);
-    const bool many_rows = o.num_rows * 4ull > kMostShared;
+    const bool many_rows = o.num_rows * 4ull > kMostPlanned;
     const size_t a_owners = part(many_rows ? o.num_rows * 4ull * kPlanBlocks : 0);
     // entries of forked rows, for lists that take two launches
     const bool stages = o.max_pages > kOneLaunchColumns ||
-                        fork_smem(o.num_rows, o.num_rows) > kMostShared ||
+                        fork_smem(o.num_rows, o.num_rows) > kMostPlanned ||
                         static_cast<size_t>(o.num_rows) * o.max_pages > kOneLaunchEntries;
     const size_t a_staged =
         part(stages ? static_cast<size_t>(o.num_rows) * o.max_pages * 4 : 0);
@@ -814,7 +814,7 @@ class PagesImpl {
     OnDevice on(device_);
     const size_t smem = fork_smem(view_.num_rows, n);
     if (view_.max_pages <= kOneLaunchColumns && n * view_.max_pages <= kOneLaunchEntries &&
-        smem <= kMostShared) {
+        smem <= kMostPlanned) {
       launch(fork_columns_kernel, (view_.max_pages + kForkColumns - 1) / kForkColumns,
              kForkColumnThreads, smem, s, 1, view_, static_cast<uint32_t>(n), src, dst, arrived_);
       return;
